@@ -16,7 +16,7 @@ A cache row of 80 bytes holds 128 values in four groups of 32: 64 bytes of codes
 Element i of group g stands for m_g + d_g c_i.  A row x is stored with, in 32-bit
 arithmetic and per group, m = fp16(min x), d = fp16((max x - m) * (1/15)) and
 c = round((x - m) (1 / d)) kept within 0 .. 15 (round half to even; 0 where d is 0);
-x is first kept within the fp16 range.  Caches are [batch][kv head][capacity][80].
+x is first kept within -65408 .. 65408.  Caches are [batch][kv head][capacity][80].
 """
 import math
 
@@ -28,7 +28,7 @@ own = False
 D = 128          # head dimension
 GROUP = 32       # elements that share a scale
 ROW = 80         # bytes of a cache row
-F16_MAX = 65504.0
+LIMIT = 65408.0  # rows are kept within this, so that m + 15 d stays an fp16 value whatever d rounds to
 
 _TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 
@@ -152,7 +152,7 @@ def work(case):
 
 def _quantize(x):
     """Rows [..., 128] to cache rows [..., 80]."""
-    x = x.float().clamp(-F16_MAX, F16_MAX).unflatten(-1, (D // GROUP, GROUP))
+    x = x.float().clamp(-LIMIT, LIMIT).unflatten(-1, (D // GROUP, GROUP))
     m = x.amin(-1, keepdim=True).half()
     d = ((x.amax(-1, keepdim=True) - m.float()) * (1.0 / 15.0)).half()
     inv = torch.where(d > 0, 1.0 / d.float(), torch.zeros_like(d, dtype=torch.float32))
@@ -338,7 +338,7 @@ def run(state):
 def _exact_rows(x):
     """What the cache holds for fp32 rows x [..., 128] (numpy), in 64 bits: the codes are chosen in the 32-bit
     arithmetic that the format prescribes."""
-    x = np.clip(x.astype(np.float32), -F16_MAX, F16_MAX)
+    x = np.clip(x.astype(np.float32), -LIMIT, LIMIT)
     out = np.empty(x.shape, np.float64)
     for g in range(0, D, GROUP):
         y = x[..., g:g + GROUP]
