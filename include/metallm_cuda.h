@@ -361,6 +361,78 @@ int mlm_attn_decode(mlm_ctx *ctx, const void *q_f16, const void *k_cache_f16,
                     int seq_len, void *out_f16);
 
 /* ---------------------------------------------------------------------------
+ * The KV cache in 4 bits: 80 bytes instead of 256 per key or value row
+ * (head_dim 128).  No counterpart in the reference, whose cache is fp16
+ * (LlamaRunner.swift:44-81); these calls stand beside the fp16 append
+ * (mlm_rope_qk_kv_append) and attention (mlm_attn_decode) for contexts and
+ * batches whose fp16 cache would not fit.
+ *
+ * A row holds 128 values in four groups of 32: bytes 0-63 are the codes
+ * (element i in byte i/2, the low nibble when i is even), bytes 64-79 four
+ * fp16 pairs (d, m).  Element i of group g stands for m[g] + d[g] * code[i].
+ * Quantization, in fp32 and per group of the input x (kept within +-65408):
+ * m = fp16(min x), d = fp16((max x - m) * (1/15)), code = round((x - m) *
+ * (1/d)), halves to even, kept within 0 .. 15 (0 where d is 0).  A group
+ * that holds a NaN has m = d = NaN.
+ *
+ * Positions, lengths and counts are int32 arrays of one entry per sequence in
+ * device memory, so a captured graph can be replayed while they grow.  Values
+ * outside the cache do not fault: rows beyond the capacity are skipped,
+ * lengths and counts are kept within their range, and mlm_wait reports
+ * MLM_ERR_SHAPE.
+ * ------------------------------------------------------------------------ */
+
+#define MLM_KV4_ROW_BYTES 80
+#define MLM_KV4_MAX_BATCH 1024
+
+/* element types of rows handed to and from the calls below (ggml_type values) */
+#define MLM_TYPE_F32 0
+#define MLM_TYPE_F16 1
+#define MLM_TYPE_BF16 30
+
+/* A caller-owned cache of one layer: k and v are [batch][n_kv_heads]
+ * [capacity] rows of MLM_KV4_ROW_BYTES, 16-byte aligned; head_dim 128; batch
+ * at most MLM_KV4_MAX_BATCH. */
+typedef struct mlm_kv4_cache {
+  void *k, *v;
+  int32_t batch, n_kv_heads, head_dim, capacity;
+} mlm_kv4_cache;
+
+/* Append key and value rows (keys already rotated, mlm_rope_f16).  k and v
+ * are [batch][tokens] rows of n_kv_heads * 128 elements of `type` (MLM_TYPE_F32,
+ * F16 or BF16), row_stride elements apart (more than n_kv_heads * 128 where
+ * they lie inside a fused QKV projection).  Row t of sequence b goes to cache
+ * row pos_dev[b] + t; with counts_dev (NULL: every sequence has `tokens`) only
+ * t < counts_dev[b].  k, v and row_stride 16-byte aligned; tokens at most the
+ * capacity. */
+int mlm_kv4_append(mlm_ctx *ctx, const mlm_kv4_cache *cache, const void *k, const void *v, int type,
+                   int64_t row_stride, int tokens, const int32_t *pos_dev,
+                   const int32_t *counts_dev);
+
+/* Read cache rows back as the fp16 rounding of the values they stand for: the
+ * rows mlm_kv4_append writes for the same tokens, pos_dev and counts_dev into
+ * k_out and v_out, fp16 [batch][tokens][n_kv_heads][128] (16-byte aligned).
+ * Rows at and past counts_dev[b], or outside the cache, are left as they were. */
+int mlm_kv4_read_f16(mlm_ctx *ctx, const mlm_kv4_cache *cache, int tokens, const int32_t *pos_dev,
+                     const int32_t *counts_dev, void *k_out_f16, void *v_out_f16);
+
+/* Grouped-query attention over the cache, causal, for `tokens` new tokens of
+ * every sequence (1: a decode step; a few: drafted tokens; many: a prompt
+ * chunk): out = softmax(q K^T / sqrt(128)) V with K and V the values the rows
+ * stand for.  Sequence b holds len_dev[b] rows, its new tokens' rows the last
+ * ones; with counts_dev (NULL: `tokens` each) its tokens are t <
+ * counts_dev[b], and token t attends to the first len - count + t + 1 rows.  A
+ * token that attends to no row gets zeros; out rows at and past counts_dev[b]
+ * are left as they were.  q fp16 and out (out_type MLM_TYPE_F16 or BF16)
+ * [batch][tokens][n_heads][128], 16-byte aligned; n_heads a multiple of
+ * n_kv_heads.  Scores, softmax statistics and sums are fp32.  Uses the
+ * context's attention scratch: launches on one context are stream-ordered and
+ * must not overlap. */
+int mlm_attn_kv4(mlm_ctx *ctx, const mlm_kv4_cache *cache, const void *q_f16, int n_heads,
+                 int tokens, const int32_t *len_dev, const int32_t *counts_dev, void *out,
+                 int out_type);
+
+/* ---------------------------------------------------------------------------
  * Embedding / argmax (the greedy loop of ContentView.swift:124-146, 274-343)
  * ------------------------------------------------------------------------ */
 
@@ -370,6 +442,36 @@ int mlm_embed_f16(mlm_ctx *ctx, const void *table_f16, int vocab, int dim,
                   const int32_t *token_dev, float *out);
 /* index of the largest logit (first on ties), written to *out_index (device) */
 int mlm_argmax_f32(mlm_ctx *ctx, const float *logits, int n, int32_t *out_index_dev);
+
+/* Settings of one row of mlm_sample_f32.  temperature <= 0 or NaN: the
+ * argmax.  top_k <= 0 or >= n: off.  top_p >= 1 or NaN: off; <= 0: the first
+ * token alone.  min_p <= 0 or NaN: off; above 1: as 1. */
+typedef struct mlm_sample_params {
+  float temperature;
+  int32_t top_k;
+  float top_p;
+  float min_p;
+} mlm_sample_params;
+
+/* One token per row of logits [rows][n] (rows row_stride floats apart), by
+ * given random numbers: the sampling beside mlm_argmax_f32 (the reference
+ * takes the argmax, ContentView.swift:124-146).  With w_i = exp((logit_i -
+ * max) / temperature) and the tokens ordered by falling logit (the lower
+ * index first among equals): keep the first top_k; of those the shortest
+ * prefix whose mass reaches top_p times theirs; of those the ones with w_i >=
+ * min_p.  The token is the first, by index, at which the running mass of the
+ * kept ones exceeds uniform_dev[row] times their sum (uniform in [0, 1);
+ * values outside are taken as the nearest inside, NaN as 0).  prob_out_dev
+ * (may be NULL) receives w of the token over the kept sum.  Weights are
+ * computed in fp64 and summed as integers (a token lighter than 2^-38 of the
+ * heaviest may be left out), so a row's result does not depend on the other
+ * rows or on the run.  NaN logits are never chosen; where a logit is +inf only
+ * such tokens weigh; a row with no logit above -inf gives mlm_argmax_f32's
+ * token, with prob 0.  n at most 2^22; params, uniforms and outputs in device
+ * memory. */
+int mlm_sample_f32(mlm_ctx *ctx, const float *logits, int rows, int n, int64_t row_stride,
+                   const mlm_sample_params *params_dev, const float *uniform_dev,
+                   int32_t *tokens_out_dev, float *prob_out_dev);
 
 /* ---------------------------------------------------------------------------
  * Tensor parallelism over NCCL, one context (one process) per GPU.  No

@@ -14,8 +14,9 @@ from typing import Optional, Sequence
 
 import numpy as np
 
-from ._lib import (LIB_PATH, TYPE_Q4_K, TYPE_Q6_K, LlamaConfig, LlamaGlobals,  # noqa: F401
-                   LlamaLayer, LlamaTypes, MLMError, RopeArgs, load, rope_args)
+from ._lib import (KV4_ROW_BYTES, LIB_PATH, TYPE_BF16, TYPE_F16, TYPE_F32, TYPE_Q4_K,  # noqa: F401
+                   TYPE_Q6_K, Kv4Cache, LlamaConfig, LlamaGlobals, LlamaLayer, LlamaTypes, MLMError,
+                   RopeArgs, SampleParams, load, rope_args)
 
 QK_K = 256
 Q4K_BLOCK_BYTES = 144
@@ -233,6 +234,53 @@ class Context:
 
     def q6k_gemv(self, W, rows: int, cols: int, x, y, residual=None) -> None:
         self.call("mlm_q6k_gemv", W, rows, cols, x, y, residual)
+
+    # -- the 4-bit KV cache and sampling ---------------------------------------
+    # Buffers are DeviceBuffers or device addresses.
+    def kv4_cache(self, batch: int, n_kv_heads: int, capacity: int) -> "Kv4Buffers":
+        """A cache of head dimension 128 in memory of its own."""
+        return Kv4Buffers(self, batch, n_kv_heads, capacity)
+
+    def kv4_append(self, cache: Kv4Cache, k, v, type: int, row_stride: int, tokens: int, pos,
+                   counts=None) -> None:
+        """Quantize K and V rows into the cache from row pos[b] on."""
+        self.call("mlm_kv4_append", cache, k, v, type, row_stride, tokens, pos, counts)
+
+    def kv4_read_f16(self, cache: Kv4Cache, tokens: int, pos, counts, k_out, v_out) -> None:
+        """The fp16 values that cache rows pos[b] .. stand for."""
+        self.call("mlm_kv4_read_f16", cache, tokens, pos, counts, k_out, v_out)
+
+    def attn_kv4(self, cache: Kv4Cache, q, n_heads: int, tokens: int, lengths, counts, out,
+                 out_type: int = TYPE_F16) -> None:
+        """Causal grouped-query attention of `tokens` new tokens per sequence."""
+        self.call("mlm_attn_kv4", cache, q, n_heads, tokens, lengths, counts, out, out_type)
+
+    def sample_f32(self, logits, rows: int, n: int, row_stride: int, params, uniform, tokens_out,
+                   prob_out=None) -> None:
+        """One token per row of logits by temperature, top-k, top-p and min-p."""
+        self.call("mlm_sample_f32", logits, rows, n, row_stride, params, uniform, tokens_out,
+                  prob_out)
+
+
+class Kv4Buffers(Kv4Cache):
+    """A Kv4Cache with device memory of its own (Context.kv4_cache)."""
+
+    def __init__(self, ctx: Context, batch: int, n_kv_heads: int, capacity: int):
+        nbytes = batch * n_kv_heads * capacity * KV4_ROW_BYTES
+        self.k_buffer, self.v_buffer = ctx.alloc(nbytes), ctx.alloc(nbytes)
+        super().__init__(self.k_buffer.ptr, self.v_buffer.ptr, batch, n_kv_heads, 128, capacity)
+
+    def free(self) -> None:
+        self.k_buffer.free()
+        self.v_buffer.free()
+        self.k = self.v = None
+
+
+def sample_params(rows: Sequence[tuple]) -> np.ndarray:
+    """(temperature, top_k, top_p, min_p) per row as the array mlm_sample_f32 reads."""
+    return np.array([tuple(r) for r in rows], dtype=[("temperature", np.float32),
+                                                     ("top_k", np.int32), ("top_p", np.float32),
+                                                     ("min_p", np.float32)])
 
 
 class Graph:

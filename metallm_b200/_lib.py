@@ -61,6 +61,24 @@ class LlamaGlobals(ctypes.Structure):
 
 
 TYPE_Q4_K, TYPE_Q6_K = 12, 14  # MLM_TYPE_*: the ggml_type values
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30
+
+
+class Kv4Cache(ctypes.Structure):
+    """mlm_kv4_cache: one layer's caller-owned 4-bit cache; k and v are device
+    addresses of [batch][n_kv_heads][capacity] rows of KV4_ROW_BYTES."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("batch", ctypes.c_int32),
+                ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("capacity", ctypes.c_int32)]
+
+
+KV4_ROW_BYTES = 80
+
+
+class SampleParams(ctypes.Structure):
+    """mlm_sample_params: one row's sampling settings."""
+    _fields_ = [("temperature", c_float), ("top_k", ctypes.c_int32), ("top_p", c_float),
+                ("min_p", c_float)]
 
 
 class LlamaTypes(ctypes.Structure):
@@ -135,6 +153,12 @@ SIGNATURES = [
     ("mlm_silu_mul_scaled", c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_int]),
     ("mlm_add_f32", c_int, [c_vp, c_vp, c_vp, c_vp, c_int]),
     ("mlm_attn_decode", c_int, [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp]),
+    ("mlm_kv4_append", c_int, [c_vp, ctypes.POINTER(Kv4Cache), c_vp, c_vp, c_int, ctypes.c_int64,
+                               c_int, c_vp, c_vp]),
+    ("mlm_kv4_read_f16", c_int, [c_vp, ctypes.POINTER(Kv4Cache), c_int, c_vp, c_vp, c_vp, c_vp]),
+    ("mlm_attn_kv4", c_int, [c_vp, ctypes.POINTER(Kv4Cache), c_vp, c_int, c_int, c_vp, c_vp, c_vp,
+                             c_int]),
+    ("mlm_sample_f32", c_int, [c_vp, c_vp, c_int, c_int, ctypes.c_int64, c_vp, c_vp, c_vp, c_vp]),
     ("mlm_embed_f16", c_int, [c_vp, c_vp, c_int, c_int, c_vp, c_vp]),
     ("mlm_argmax_f32", c_int, [c_vp, c_vp, c_int, c_vp]),
     ("mlm_llama_create", c_int, [c_vp, ctypes.POINTER(LlamaConfig), ctypes.POINTER(c_vp)]),

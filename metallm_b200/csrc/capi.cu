@@ -136,7 +136,8 @@ extern "C" int mlm_create(int device, mlm_ctx **out) {
   }
   if (gemv_init(ctx) != MLM_OK || attn_init(ctx) != MLM_OK ||
       gemm_init(ctx) != MLM_OK || prefill_init(ctx) != MLM_OK ||
-      gemv_batch_init(ctx) != MLM_OK || q6k_init(ctx) != MLM_OK)
+      gemv_batch_init(ctx) != MLM_OK || q6k_init(ctx) != MLM_OK ||
+      kv4_attn_init(ctx) != MLM_OK || sample_init(ctx) != MLM_OK)
     return fail(MLM_ERR_CUDA);
   if (cudaDeviceSynchronize() != cudaSuccess) return fail(MLM_ERR_CUDA);
   *out = ctx;
@@ -261,6 +262,10 @@ extern "C" int mlm_wait(mlm_ctx *ctx) {
   const int dev = *ctx->host_status;
   if (dev != 0) {
     *ctx->host_status = 0;
+    if (dev == MLM_ERR_SHAPE)
+      return set_error(ctx, dev,
+                       "command buffer failed: a position, length or count in device memory lies "
+                       "outside its cache");
     return set_error(ctx, dev, "command buffer failed: a kernel's bounded wait expired (%s)",
                      mlm_status_string(dev));
   }

@@ -67,6 +67,10 @@ namespace mlm {
 int set_error(mlm_ctx *ctx, int code, const char *fmt, ...)
     __attribute__((format(printf, 3, 4)));
 int check_launch(mlm_ctx *ctx, const char *what);
+int kv4_attn_init(mlm_ctx *ctx);  // kv4_attn.cu: shared-memory limits, scratch
+int sample_init(mlm_ctx *ctx);    // sample.cu: shared-memory and cluster limits
+// kv4.cu: the checks every call on a 4-bit cache makes of it
+int kv4_check(mlm_ctx *ctx, const mlm_kv4_cache *cache, const char *what);
 int q6k_init(mlm_ctx *ctx);  // q6k.cu: the GEMV's shared-memory limit
 struct GemvInput;
 // the Q6_K decode GEMV with the Q4_K GEMV's x modes (cols a multiple of 2048)
@@ -228,6 +232,25 @@ int tp_allgather_bytes(mlm_ctx *ctx, const void *send, void *recv, size_t bytes,
 void tp_destroy(mlm_ctx *ctx);
 int embed_launch(mlm_ctx *ctx, const void *table, int vocab, int dim, const int32_t *tok,
                  float *out, cudaStream_t stream);
+
+// makes the context's device current for a call and restores the caller's
+class DeviceGuard {
+ public:
+  explicit DeviceGuard(const mlm_ctx *ctx) {
+    if (cudaGetDevice(&saved_) != cudaSuccess) saved_ = ctx->device;
+    if (saved_ != ctx->device) cudaSetDevice(ctx->device);
+    changed_ = saved_ != ctx->device;
+  }
+  ~DeviceGuard() {
+    if (changed_) cudaSetDevice(saved_);
+  }
+  DeviceGuard(const DeviceGuard &) = delete;
+  DeviceGuard &operator=(const DeviceGuard &) = delete;
+
+ private:
+  int saved_ = 0;
+  bool changed_ = false;
+};
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
