@@ -233,6 +233,9 @@ int kv4_check(mlm_ctx *ctx, const mlm_kv4_cache *c, const char *what) {
                        c->capacity <= (1 << 30),
               MLM_ERR_SHAPE, "%s: n_kv_heads=%d (1 .. 1024) capacity=%d (1 .. 2^30)", what,
               c->n_kv_heads, c->capacity);
+  MLM_REQUIRE(ctx, (long long)c->batch * c->n_kv_heads * c->capacity <= (1ll << 32), MLM_ERR_SHAPE,
+              "%s: batch=%d x n_kv_heads=%d x capacity=%d rows (at most 2^32)", what, c->batch,
+              c->n_kv_heads, c->capacity);
   MLM_REQUIRE(ctx, aligned16(c->k) && aligned16(c->v), MLM_ERR_ALIGN,
               "%s: the cache must be 16-byte aligned", what);
   return MLM_OK;

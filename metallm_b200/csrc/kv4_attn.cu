@@ -4,18 +4,649 @@
 // and V the values m + d c the cache rows stand for (the fp16 cache's
 // counterpart is mlm_attn_decode; LlamaRunner.swift:669-952).
 //
-// One warp per (sequence, token, query head) walks the rows the token sees with
-// a running maximum and sum; a lane holds dimensions 4l .. 4l+3.
+// Pointers to data that earlier kernels write carry no __restrict__, so that no
+// load of it moves above the dependent wait.
 #include <algorithm>
 
 #include "mlm_device.cuh"
 #include "mlm_internal.h"
+#include "q4k_gemv_common.cuh"
 
 namespace mlm {
 namespace {
 
 constexpr int kRow = MLM_KV4_ROW_BYTES;
 constexpr int kD = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInvSqrtD = 0.08838834764831845f;
+
+// ---------------------------------------------------------------------------
+// Few rows: up to 16 (token, head) pairs of one KV head at once -- a decode
+// step, a few drafted tokens.  Bound by the cache's bytes (160 per position
+// and KV head), then by instruction issue.
+//
+// Both products run on the tensor cores on the codes themselves.  A masked
+// nibble in a binary16's low mantissa bits is the subnormal c 2^-24 (16 c
+// 2^-24 one nibble up), so one AND makes two operands; the group's d and m,
+// constant along the 32 elements of a group, enter outside the product:
+//   q.k = sum_g d_g (sum_i q_i c_i) + m_g (sum_i q_i)
+//   o_i = sum_j (p_j d_jg) c_ji + sum_j p_j m_jg
+// K is the A operand (16 rows x 16 dimensions), the queries the 8 columns of
+// B; V^T is the A operand (16 dimensions x 16 rows; ldmatrix.trans of the codes
+// as 16-bit units hands a lane the nibbles of two neighbouring rows side by
+// side), the weights p d the 8 columns of B.  Nothing of K or V is rounded; q is
+// fp16 already (scaled by a power of two per row, so that q / 16 stays exact);
+// p d goes in as fp16 hi + lo.  With at most four columns the hi and lo parts
+// share the eight columns of one product.  Scores, statistics and sums are fp32.
+//
+// Work is cut by bytes, not by head: the blocks of 32 rows of every (sequence,
+// KV head) form one line, cut into equal stretches per CTA and again per warp
+// from the lengths in device memory, so ragged batches and graph replays stay
+// balanced.  A warp streams its blocks through a ring of its own (two 2560-byte
+// bulk copies per block, contiguous in the cache) and keeps a running maximum
+// and sum per column.  Stretches of one head are joined in order: a warp's
+// pieces in shared memory, a CTA's through the context's scratch by the last
+// CTA of the head to arrive, so sums do not depend on timing.
+// ---------------------------------------------------------------------------
+
+constexpr int kBlk = 32;                     // cache rows per block
+constexpr int kHalfStage = kBlk * kRow;      // K or V of a block
+constexpr int kStage = 2 * kHalfStage;
+constexpr int kPieceRow = kD + 2;            // a column of a piece: o[128], m, l
+constexpr int kMaxCols = 16;
+
+struct FewArgs {
+  const uint8_t *kc, *vc;
+  const __half *q;
+  void *out;
+  const int32_t *lens, *counts;
+  float *parts;   // [ctas][2][kMaxCols][kPieceRow]
+  int *arrivals;  // [ctas], zero between launches
+  int *status;
+  int batch, tokens, n_heads, n_kv, group, capacity;
+};
+
+// the sequence's rows and tokens, kept within the cache and the call
+__device__ __forceinline__ void seq_shape(const int32_t *lens, const int32_t *counts, int b,
+                                          int tokens, int capacity, int &len, int &count) {
+  len = min(max(lens[b], 0), capacity);
+  count = counts ? min(max(counts[b], 0), tokens) : tokens;
+}
+__device__ __forceinline__ bool seq_outside(const int32_t *lens, const int32_t *counts, int b,
+                                            int tokens, int capacity) {
+  return lens[b] < 0 || lens[b] > capacity || (counts && (counts[b] < 0 || counts[b] > tokens));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+// the transpose of an 8x8 matrix of 16-bit elements, row r of it in lanes 4r ..
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t u4_get(const uint4 &v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+// a position on the line of blocks
+struct Cursor {
+  int b, h, blk, nb;  // block blk of nb of (b, h)
+};
+
+template <int NT, bool DUP, int W, int STAGES, class OutT>
+__global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
+  static_assert(!DUP || NT == 1, "hi and lo share one tile of columns");
+  constexpr int kCols = DUP ? 4 : 8 * NT;
+  constexpr int kPiece = kCols * kPieceRow;
+  static_assert(kPiece * 4 <= STAGES * kStage, "a warp's last piece lies in its ring");
+  extern __shared__ __align__(128) uint8_t smem[];
+  // rings, the warps' head pieces, the line's offsets per sequence
+  float *s_head = reinterpret_cast<float *>(smem + W * STAGES * kStage);
+  int *s_off = reinterpret_cast<int *>(s_head + W * kPiece);  // [batch + 1]
+  __shared__ __align__(8) uint64_t s_bar[W][STAGES];
+  __shared__ int s_item[2 * W], s_bh[2 * W];  // pieces: the item's first block (-1: none), b and h
+  __shared__ int s_last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r = lane >> 2, t4 = lane & 3;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * kStage;
+  const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(&s_bar[warp][0]);
+  if (lane == 0) {
+    for (int i = 0; i < STAGES; ++i) mbar_init(bar0 + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x < 2 * W) s_item[threadIdx.x] = -1;
+  pdl_wait_then_release();
+
+  // the line's offsets: sequence b's blocks start at s_off[b]
+  if (warp == 0) {
+    int run = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+      const int b = b0 + lane;
+      int n = 0;
+      if (b < a.batch) {
+        int len, count;
+        seq_shape(a.lens, a.counts, b, a.tokens, a.capacity, len, count);
+        n = count > 0 ? (len + kBlk - 1) / kBlk * a.n_kv : 0;
+        if (blockIdx.x == 0 && seq_outside(a.lens, a.counts, b, a.tokens, a.capacity))
+          *a.status = MLM_ERR_SHAPE;
+      }
+      int in = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, in, o);
+        if (lane >= o) in += up;
+      }
+      if (b < a.batch) s_off[b] = run + in - n;
+      run += __shfl_sync(0xffffffffu, in, 31);
+    }
+    if (lane == 0) s_off[a.batch] = run;
+  }
+  __syncthreads();
+  const int total = s_off[a.batch];
+  // tokens that attend to nothing in sequences without blocks
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    if (s_off[b + 1] > s_off[b]) continue;
+    int len, count;
+    seq_shape(a.lens, a.counts, b, a.tokens, a.capacity, len, count);
+    OutT *o = reinterpret_cast<OutT *>(a.out) + (size_t)b * a.tokens * a.n_heads * kD;
+    for (int i = threadIdx.x; i < count * a.n_heads * kD; i += W * 32) o[i] = from_float<OutT>(0.f);
+  }
+  // equal stretches, at least one block per warp
+  const int quota = max(W, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  const int cta0 = min(total, (int)blockIdx.x * quota), cta1 = min(total, cta0 + quota);
+  if (cta0 >= cta1) return;
+  const int w0 = cta0 + (cta1 - cta0) * warp / W, w1 = cta0 + (cta1 - cta0) * (warp + 1) / W;
+
+  auto at = [&](int x) {
+    int lo = 0, hi = a.batch;  // the last b with s_off[b] <= x
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_off[mid] <= x) lo = mid; else hi = mid;
+    }
+    Cursor c;
+    c.b = lo;
+    c.nb = (s_off[lo + 1] - s_off[lo]) / a.n_kv;
+    const int rem = x - s_off[lo];
+    c.h = rem / c.nb;
+    c.blk = rem - c.h * c.nb;
+    return c;
+  };
+  auto next = [&](Cursor &c) {
+    if (++c.blk < c.nb) return;
+    c.blk = 0;
+    if (++c.h < a.n_kv) return;
+    c.h = 0;
+    do ++c.b; while (c.b < a.batch && s_off[c.b + 1] == s_off[c.b]);
+    if (c.b < a.batch) c.nb = (s_off[c.b + 1] - s_off[c.b]) / a.n_kv;
+  };
+  auto issue = [&](const Cursor &c, int stage) {  // one lane
+    int len, count;
+    seq_shape(a.lens, a.counts, c.b, a.tokens, a.capacity, len, count);
+    const uint32_t bytes = (uint32_t)min(kBlk, len - c.blk * kBlk) * kRow;
+    const size_t off = (((size_t)c.b * a.n_kv + c.h) * a.capacity + (size_t)c.blk * kBlk) * kRow;
+    const uint32_t bar = bar0 + 8 * stage, dst = ring + stage * kStage;
+    mbar_expect_tx(bar, 2 * bytes);
+    bulk_copy(dst, a.kc + off, bytes, bar);
+    bulk_copy(dst + kHalfStage, a.vc + off, bytes, bar);
+  };
+
+  Cursor cur = {}, ahead = {};
+  int issued = w0;
+  if (w0 < w1) {
+    cur = ahead = at(w0);
+    for (; issued < min(w1, w0 + STAGES); ++issued) {
+      if (lane == 0) issue(ahead, issued - w0);
+      next(ahead);
+    }
+  }
+
+  // queries: the B operand of K's products, per group of 32 dimensions
+  uint32_t qb[NT][4][4];
+  float qs[NT][4][2];          // sums of the scaled q over a group, columns 2 t4, 2 t4 + 1
+  float cs[NT];                // score scale of column r, in powers of two
+  int seen[NT];                // rows column r attends to
+  int len = 0, count = 0, seen_min = 0;
+  float o[NT][4][2][4], om[NT][4], mx[NT], l[NT];
+  bool ok = true;
+  int first = w0;              // where the current item starts within this warp's stretch
+
+  for (int x = w0; x < w1; ++x) {
+    if (x == w0 || cur.blk == 0) {
+      first = x;
+      seq_shape(a.lens, a.counts, cur.b, a.tokens, a.capacity, len, count);
+      seen_min = max(0, len - count + 1);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int col = DUP ? (r & 3) : nt * 8 + r;
+        const bool live = col < count * a.group;
+        const int tok = live ? col / a.group : 0;
+        seen[nt] = live ? max(0, len - count + tok + 1) : 0;
+        const __half *qr = a.q + (((size_t)cur.b * a.tokens + tok) * a.n_heads +
+                                  cur.h * a.group + (col - tok * a.group)) * kD + 8 * t4;
+        float f[4][8], big = 0.f;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const uint4 v = live ? *reinterpret_cast<const uint4 *>(qr + 32 * g) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 p = unpack_f16(u4_get(v, i));
+            f[g][2 * i] = p.x;
+            f[g][2 * i + 1] = p.y;
+            big = fmaxf(big, fmaxf(fabsf(p.x), fabsf(p.y)));
+          }
+        }
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        // the largest |q| of the row into [2^13, 2^14): q / 16 keeps its bits
+        const int e = big > 0.f ? 13 - ((int)((__float_as_uint(big) >> 23) & 0xFF) - 127) : 0;
+        const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+        cs[nt] = kInvSqrtD * kLog2e * __uint_as_float((uint32_t)(24 - e + 127) << 23);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            f[g][i] *= up;
+            sum += f[g][i];
+          }
+          qb[nt][g][0] = pack_f16(f[g][0], f[g][4]);
+          qb[nt][g][1] = pack_f16(f[g][1] * 0.0625f, f[g][5] * 0.0625f);
+          qb[nt][g][2] = pack_f16(f[g][2], f[g][6]);
+          qb[nt][g][3] = pack_f16(f[g][3] * 0.0625f, f[g][7] * 0.0625f);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          sum *= 5.9604644775390625e-08f;  // 2^-24, the codes' unit
+          qs[nt][g][0] = __shfl_sync(0xffffffffu, sum, 8 * t4);
+          qs[nt][g][1] = __shfl_sync(0xffffffffu, sum, 8 * t4 + 4);
+          om[nt][g] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[nt][g][0][i] = o[nt][g][1][i] = 0.f;
+        }
+        mx[nt] = -INFINITY;
+        l[nt] = 0.f;
+      }
+    }
+    const int stage = (x - w0) % STAGES;
+    const uint32_t sk = ring + stage * kStage, sv = sk + kHalfStage;
+    ok = mbar_wait_bounded(bar0 + 8 * stage, (uint32_t)((x - w0) / STAGES) & 1, a.status);
+    if (!__all_sync(0xffffffffu, ok)) {
+      ok = false;
+      break;
+    }
+
+    // scores of the block's two 16-row tiles
+    const uint32_t tile_lane = (uint32_t)((((lane >> 3) & 1) * 8 + (lane & 7)) * kRow + (lane >> 4) * 16);
+    float sT[NT][2][2][2];  // column r: rows 16 kt + 8 half + 2 t4 + {0, 1}
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      uint32_t w[2][4];
+      ldsm4(sk + kt * 16 * kRow + tile_lane, w[0]);
+      ldsm4(sk + kt * 16 * kRow + tile_lane + 32, w[1]);
+      const uint4 dm0 = lds16(sk + (kt * 16 + r) * kRow + 64);
+      const uint4 dm1 = lds16(sk + (kt * 16 + r + 8) * kRow + 64);
+      float s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t wa = w[g >> 1][(g & 1) * 2], wb = w[g >> 1][(g & 1) * 2 + 1];
+        const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
+        const float2 f0 = unpack_f16(u4_get(dm0, g)), f1 = unpack_f16(u4_get(dm1, g));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_f16_16816(acc, wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u,
+                        wb & 0x00F000F0u, qb[nt][g][0], qb[nt][g][1]);
+          mma_f16_16816(acc, wa8 & 0x000F000Fu, wb8 & 0x000F000Fu, wa8 & 0x00F000F0u,
+                        wb8 & 0x00F000F0u, qb[nt][g][2], qb[nt][g][3]);
+          s[nt][0] = fmaf(f0.x, acc[0], fmaf(f0.y, qs[nt][g][0], s[nt][0]));
+          s[nt][1] = fmaf(f0.x, acc[1], fmaf(f0.y, qs[nt][g][1], s[nt][1]));
+          s[nt][2] = fmaf(f1.x, acc[2], fmaf(f1.y, qs[nt][g][0], s[nt][2]));
+          s[nt][3] = fmaf(f1.x, acc[3], fmaf(f1.y, qs[nt][g][1], s[nt][3]));
+        }
+      }
+      // rows x columns to columns x rows, as the V product's B operand wants
+      // the weights: 32-bit values as two 16-bit matrices
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t v0 = __float_as_uint(s[nt][2 * half]), v1 = __float_as_uint(s[nt][2 * half + 1]);
+          const uint32_t lo = transpose8(__byte_perm(v0, v1, 0x5410));
+          const uint32_t hi = transpose8(__byte_perm(v0, v1, 0x7632));
+          sT[nt][kt][half][0] = cs[nt] * __uint_as_float(__byte_perm(lo, hi, 0x5410));
+          sT[nt][kt][half][1] = cs[nt] * __uint_as_float(__byte_perm(lo, hi, 0x7632));
+        }
+    }
+    const int row0 = cur.blk * kBlk + 2 * t4;  // this lane's first row of the block
+    const bool masked = (cur.blk + 1) * kBlk > seen_min;  // uniform in the warp
+    if (masked) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (row0 + (i >> 2) * 16 + ((i >> 1) & 1) * 8 + (i & 1) >= seen[nt])
+            sT[nt][i >> 2][(i >> 1) & 1][i & 1] = -INFINITY;
+    }
+    // running maximum and sum; the weights carry a factor of 4 (p <= 4), which
+    // l carries too: p d stays an fp16 value for every d below 2^14
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float top = mx[nt];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, sT[nt][i >> 2][(i >> 1) & 1][i & 1]);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      if (__any_sync(0xffffffffu, top != mx[nt])) {
+        const float f = top == mx[nt] ? 1.f : ex2(mx[nt] - top);
+        l[nt] *= f;
+        const float f0 = __shfl_sync(0xffffffffu, f, 8 * t4), f1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          om[nt][g] *= f;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            o[nt][g][i][0] *= f0;
+            o[nt][g][i][1] *= f1;
+            o[nt][g][i][2] *= f0;
+            o[nt][g][i][3] *= f1;
+          }
+        }
+        mx[nt] = top;
+      }
+      const float base = (top == -INFINITY ? 0.f : top) - 2.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float &v = sT[nt][i >> 2][(i >> 1) & 1][i & 1];
+        v = ex2(v - base);
+        l[nt] += v;
+      }
+    }
+    // o += (p d) c and the m part
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      uint32_t w[2][4];
+      ldsm4_t(sv + kt * 16 * kRow + tile_lane, w[0]);
+      ldsm4_t(sv + kt * 16 * kRow + tile_lane + 32, w[1]);
+      uint4 dm[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        dm[i] = lds16(sv + (kt * 16 + (i >> 1) * 8 + 2 * t4 + (i & 1)) * kRow + 64);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t wa = w[g >> 1][(g & 1) * 2], wb = w[g >> 1][(g & 1) * 2 + 1];
+        const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
+        float2 f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = unpack_f16(u4_get(dm[i], g));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = sT[nt][kt][i >> 1][i & 1];
+            v[i] = p * f[i].x;
+            float pm = p * f[i].y;
+            // a row this column does not see adds nothing, whatever its scales hold
+            if (masked && row0 + kt * 16 + (i >> 1) * 8 + (i & 1) >= seen[nt]) v[i] = pm = 0.f;
+            om[nt][g] += pm;
+          }
+          uint32_t b0 = pack_f16(v[0], v[1]), b1 = pack_f16(v[2], v[3]);
+          const float2 h0 = unpack_f16(b0), h1 = unpack_f16(b1);
+          const uint32_t l0 = pack_f16(v[0] - h0.x, v[1] - h0.y), l1 = pack_f16(v[2] - h1.x, v[3] - h1.y);
+          if (DUP && r >= 4) {
+            b0 = l0;
+            b1 = l1;
+          }
+          mma_f16_16816(o[nt][g][0], wa & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x000F000Fu,
+                        wb & 0x00F000F0u, b0, b1);
+          mma_f16_16816(o[nt][g][1], wa8 & 0x000F000Fu, wa8 & 0x00F000F0u, wb8 & 0x000F000Fu,
+                        wb8 & 0x00F000F0u, b0, b1);
+          if (!DUP) {
+            mma_f16_16816(o[nt][g][0], wa & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x000F000Fu,
+                          wb & 0x00F000F0u, l0, l1);
+            mma_f16_16816(o[nt][g][1], wa8 & 0x000F000Fu, wa8 & 0x00F000F0u, wb8 & 0x000F000Fu,
+                          wb8 & 0x00F000F0u, l0, l1);
+          }
+        }
+      }
+    }
+    __syncwarp();  // every lane is done with the stage
+    if (issued < w1) {
+      if (lane == 0) issue(ahead, stage);
+      next(ahead);
+      ++issued;
+    }
+
+    // the item or the stretch ends: its output, or a piece of it
+    const bool item_ends = cur.blk + 1 == cur.nb;
+    if (item_ends || x + 1 == w1) {
+      const int item = x - cur.blk;  // the item's first block on the line
+      const bool whole = item_ends && first == item;
+      const int slot = 2 * warp + (x + 1 == w1 ? 1 : 0);
+      float *piece = x + 1 == w1 ? reinterpret_cast<float *>(smem + warp * STAGES * kStage)
+                                 : s_head + warp * kPiece;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], 1);
+        l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], 2);
+        const float inv = whole ? (l[nt] > 0.f ? 1.f / l[nt] : (l[nt] == 0.f ? 0.f : NAN)) : 1.f;
+        const float i0 = __shfl_sync(0xffffffffu, inv, 8 * t4), i1 = __shfl_sync(0xffffffffu, inv, 8 * t4 + 4);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float m = om[nt][g];
+          m += __shfl_xor_sync(0xffffffffu, m, 1);
+          m += __shfl_xor_sync(0xffffffffu, m, 2);
+          const float m0 = __shfl_sync(0xffffffffu, m, 8 * t4), m1 = __shfl_sync(0xffffffffu, m, 8 * t4 + 4);
+          float v[2][4];  // columns 2 t4 and 2 t4 + 1, dimensions 32 g + 4 r ..
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float w = o[nt][g][i][c];
+              if (DUP) w += __shfl_xor_sync(0xffffffffu, w, 2);  // hi + lo
+              // the codes' unit: 2^-24, and 16 times that in rows 8 .. 15
+              v[c & 1][2 * i + (c >> 1)] = fmaf(w, c < 2 ? 16777216.f : 1048576.f, (c & 1) ? m1 : m0);
+            }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int col = nt * 8 + 2 * t4 + c;
+            if (DUP && col >= 4) continue;
+            if (whole) {
+              if (col >= count * a.group) continue;
+              const int tok = col / a.group;
+              OutT *dst = reinterpret_cast<OutT *>(a.out) +
+                          (((size_t)cur.b * a.tokens + tok) * a.n_heads + cur.h * a.group +
+                           (col - tok * a.group)) * kD + 32 * g + 4 * r;
+              const float f = c ? i1 : i0;
+              OutT e[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) e[i] = from_float<OutT>(v[c][i] * f);
+              *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(e);
+            } else {
+              float *dst = piece + col * kPieceRow + 32 * g + 4 * r;
+#pragma unroll
+              for (int i = 0; i < 4; i += 2)
+                *reinterpret_cast<float2 *>(dst + i) = make_float2(v[c][i], v[c][i + 1]);
+            }
+          }
+        }
+        if (!whole && t4 == 0 && (!DUP || r < 4)) {
+          piece[(nt * 8 + r) * kPieceRow + kD] = mx[nt];
+          piece[(nt * 8 + r) * kPieceRow + kD + 1] = l[nt];
+        }
+      }
+      if (!whole && lane == 0) {
+        s_item[slot] = item;
+        s_bh[slot] = cur.b * a.n_kv + cur.h;
+      }
+    }
+    next(cur);
+  }
+  if (!ok)  // status is set; let this warp's copies land before its shared memory goes
+    for (int s = 0; s < STAGES && s < issued - w0; ++s)
+      mbar_wait_bounded(bar0 + 8 * s, (uint32_t)((issued - w0 - 1 - s) / STAGES) & 1, a.status);
+  __syncthreads();
+
+  // join the pieces: a run of slots holding one item at a time
+  auto piece_of = [&](int slot) -> const float * {
+    return (slot & 1) ? reinterpret_cast<const float *>(smem + (slot >> 1) * STAGES * kStage)
+                      : s_head + (slot >> 1) * kPiece;
+  };
+  auto emit = [&](int bh, int col, int d, float v) {
+    const int b = bh / a.n_kv, h = bh - b * a.n_kv;
+    int n, c;
+    seq_shape(a.lens, a.counts, b, a.tokens, a.capacity, n, c);
+    if (col >= c * a.group) return;
+    const int tok = col / a.group;
+    reinterpret_cast<OutT *>(a.out)[(((size_t)b * a.tokens + tok) * a.n_heads + h * a.group +
+                                     (col - tok * a.group)) * kD + d] = from_float<OutT>(v);
+  };
+  for (int s0 = 0; s0 < 2 * W;) {
+    const int item = s_item[s0];
+    if (item < 0) {
+      ++s0;
+      continue;
+    }
+    int s1 = s0 + 1;
+    while (s1 < 2 * W && (s_item[s1] < 0 || s_item[s1] == item)) ++s1;
+    const int bh = s_bh[s0], b = bh / a.n_kv;
+    const int nb = (s_off[b + 1] - s_off[b]) / a.n_kv;
+    const bool complete = item >= cta0 && item + nb <= cta1;
+    float *part = a.parts + ((size_t)blockIdx.x * 2 + (item < cta0 ? 0 : 1)) * kMaxCols * kPieceRow;
+    for (int i = threadIdx.x; i < kCols * kD; i += W * 32) {
+      const int col = i / kD, d = i - col * kD;
+      float top = -INFINITY;
+      for (int s = s0; s < s1; ++s)
+        if (s_item[s] >= 0) top = fmaxf(top, piece_of(s)[col * kPieceRow + kD]);
+      float sum = 0.f, v = 0.f;
+      for (int s = s0; s < s1; ++s) {
+        if (s_item[s] < 0) continue;
+        const float *p = piece_of(s) + col * kPieceRow;
+        const float f = p[kD] == top ? 1.f : ex2(p[kD] - top);
+        v += f * p[d];
+        sum += f * p[kD + 1];
+      }
+      if (complete) {
+        emit(bh, col, d, sum == 0.f ? 0.f : v / sum);
+      } else {
+        part[col * kPieceRow + d] = v;
+        if (d == 0) {
+          part[col * kPieceRow + kD] = top;
+          part[col * kPieceRow + kD + 1] = sum;
+        }
+      }
+    }
+    if (!complete) {
+      // the last CTA of the item to arrive joins the CTAs' parts, in order
+      const int c0 = item / quota, c1 = (item + nb - 1) / quota;
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const int n = atomicAdd(a.arrivals + c0, 1);
+        s_last = n == c1 - c0;
+        if (s_last) a.arrivals[c0] = 0;
+      }
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        for (int i = threadIdx.x; i < kCols * kD; i += W * 32) {
+          const int col = i / kD, d = i - col * kD;
+          auto of = [&](int c) {
+            return a.parts + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kMaxCols * kPieceRow + col * kPieceRow;
+          };
+          float top = -INFINITY;
+          for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(of(c) + kD));
+          float sum = 0.f, v = 0.f;
+#pragma unroll 4
+          for (int c = c0; c <= c1; ++c) {
+            const float m = __ldcg(of(c) + kD);
+            const float f = m == top ? 1.f : ex2(m - top);
+            v += f * __ldcg(of(c) + d);
+            sum += f * __ldcg(of(c) + kD + 1);
+          }
+          emit(bh, col, d, sum == 0.f ? 0.f : v / sum);
+        }
+      }
+      __syncthreads();
+    }
+    s0 = s1;
+  }
+}
+
+// warps and ring stages per column count: the rings hold 140-164 KB in flight
+// per SM beside the warps' head pieces
+template <int NT, bool DUP>
+struct FewShape {
+  static constexpr int warps = DUP ? 16 : NT == 1 ? 14 : 8;
+  static constexpr int stages = NT == 1 ? 2 : 3;
+  static constexpr int cols = DUP ? 4 : 8 * NT;
+  static constexpr size_t smem(int batch) {
+    return (size_t)warps * stages * kStage + (size_t)warps * cols * kPieceRow * 4 +
+           sizeof(int) * (batch + 1);
+  }
+};
+
+template <int NT, bool DUP, class OutT>
+constexpr auto few_kernel() {
+  using S = FewShape<NT, DUP>;
+  return kv4_attn_few_kernel<NT, DUP, S::warps, S::stages, OutT>;
+}
+
+template <int NT, bool DUP, class OutT>
+int few_launch(mlm_ctx *ctx, const FewArgs &a) {
+  using S = FewShape<NT, DUP>;
+  return check_launch_pdl(ctx,
+                          launch_pdl(few_kernel<NT, DUP, OutT>(), dim3(ctx->sm_count),
+                                     dim3(S::warps * 32), S::smem(a.batch), ctx->stream, a),
+                          "mlm_attn_kv4");
+}
+template <class OutT>
+int few(mlm_ctx *ctx, const FewArgs &a) {
+  const int cols = a.tokens * a.group;
+  if (cols <= 4) return few_launch<1, true, OutT>(ctx, a);
+  if (cols <= 8) return few_launch<1, false, OutT>(ctx, a);
+  return few_launch<2, false, OutT>(ctx, a);
+}
 
 // the lane's four values of a cache row
 __device__ __forceinline__ float4 row4(const uint8_t *row, int lane) {
@@ -25,6 +656,8 @@ __device__ __forceinline__ float4 row4(const uint8_t *row, int lane) {
                      fmaf(dm.x, (float)((w >> 8) & 15u), dm.y), fmaf(dm.x, (float)(w >> 12), dm.y));
 }
 
+// Many rows: one warp per (sequence, token, query head) walks the rows the token
+// sees with a running maximum and sum; a lane holds dimensions 4l .. 4l+3.
 template <class OutT>
 __global__ void __launch_bounds__(128) kv4_attn_simple_kernel(
     const uint8_t *kc, const uint8_t *vc, const __half *q, OutT *out, int batch, int tokens,
@@ -36,12 +669,9 @@ __global__ void __launch_bounds__(128) kv4_attn_simple_kernel(
   const int head = (int)(i % n_heads);
   const int t = (int)(i / n_heads % tokens);
   const int b = (int)(i / n_heads / tokens);
-  int len = lens[b], count = counts ? counts[b] : tokens;
-  if (len < 0 || len > capacity || count < 0 || count > tokens) {
-    if (lane == 0) *status = MLM_ERR_SHAPE;
-    len = min(max(len, 0), capacity);
-    count = min(max(count, 0), tokens);
-  }
+  int len, count;
+  seq_shape(lens, counts, b, tokens, capacity, len, count);
+  if (lane == 0 && seq_outside(lens, counts, b, tokens, capacity)) *status = MLM_ERR_SHAPE;
   if (t >= count) return;
   const int seen = max(0, len - count + t + 1);
   const size_t at = (size_t)i * kD + 4 * lane;
@@ -52,7 +682,7 @@ __global__ void __launch_bounds__(128) kv4_attn_simple_kernel(
   float top = -INFINITY, sum = 0.f, o[4] = {};
   for (int j = 0; j < seen; ++j) {
     const float4 k = row4(kc + (row0 + j) * kRow, lane);
-    const float s = warp_sum(x[0] * k.x + x[1] * k.y + x[2] * k.z + x[3] * k.w) * 0.08838834764831845f;
+    const float s = warp_sum(x[0] * k.x + x[1] * k.y + x[2] * k.z + x[3] * k.w) * kInvSqrtD;
     const float up = fmaxf(top, s);
     const float old = top == up ? 1.f : expf(top - up), p = expf(s - up);
     const float4 v = row4(vc + (row0 + j) * kRow, lane);
@@ -81,9 +711,31 @@ int simple(mlm_ctx *ctx, const mlm_kv4_cache &c, const void *q, int n_heads, int
       "mlm_attn_kv4");
 }
 
+template <int NT, bool DUP, class OutT>
+int few_init(mlm_ctx *ctx) {
+  MLM_CUDA_TRY(ctx, cudaFuncSetAttribute(few_kernel<NT, DUP, OutT>(),
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)FewShape<NT, DUP>::smem(MLM_KV4_MAX_BATCH)));
+  return MLM_OK;
+}
+
 }  // namespace
 
-int kv4_attn_init(mlm_ctx *) { return MLM_OK; }
+int kv4_attn_init(mlm_ctx *ctx) {
+  int st = few_init<1, true, __half>(ctx);
+  if (st == MLM_OK) st = few_init<1, false, __half>(ctx);
+  if (st == MLM_OK) st = few_init<2, false, __half>(ctx);
+  if (st == MLM_OK) st = few_init<1, true, __nv_bfloat16>(ctx);
+  if (st == MLM_OK) st = few_init<1, false, __nv_bfloat16>(ctx);
+  if (st == MLM_OK) st = few_init<2, false, __nv_bfloat16>(ctx);
+  if (st != MLM_OK) return st;
+  const size_t parts = sizeof(float) * 2 * ctx->sm_count * kMaxCols * kPieceRow;
+  if (cudaMalloc(&ctx->kv4_parts, parts) != cudaSuccess ||
+      cudaMalloc(&ctx->kv4_arrivals, sizeof(int) * ctx->sm_count) != cudaSuccess)
+    return set_error(ctx, MLM_ERR_ALLOC, "mlm_attn_kv4: scratch");
+  MLM_CUDA_TRY(ctx, cudaMemset(ctx->kv4_arrivals, 0, sizeof(int) * ctx->sm_count));
+  return MLM_OK;
+}
 
 }  // namespace mlm
 
@@ -108,6 +760,26 @@ extern "C" int mlm_attn_kv4(mlm_ctx *ctx, const mlm_kv4_cache *cache, const void
   MLM_REQUIRE(ctx, tokens > 0 && tokens <= 65536, MLM_ERR_SHAPE,
               "mlm_attn_kv4: tokens=%d (1 .. 65536)", tokens);
   DeviceGuard guard(ctx);
+  const int group = n_heads / cache->n_kv_heads;
+  if ((long long)tokens * group <= kMaxCols) {
+    FewArgs a;
+    a.kc = reinterpret_cast<const uint8_t *>(cache->k);
+    a.vc = reinterpret_cast<const uint8_t *>(cache->v);
+    a.q = reinterpret_cast<const __half *>(q);
+    a.out = out;
+    a.lens = lens;
+    a.counts = counts;
+    a.parts = ctx->kv4_parts;
+    a.arrivals = ctx->kv4_arrivals;
+    a.status = ctx->dev_status;
+    a.batch = cache->batch;
+    a.tokens = tokens;
+    a.n_heads = n_heads;
+    a.n_kv = cache->n_kv_heads;
+    a.group = group;
+    a.capacity = cache->capacity;
+    return out_type == MLM_TYPE_F16 ? few<__half>(ctx, a) : few<__nv_bfloat16>(ctx, a);
+  }
   if (out_type == MLM_TYPE_F16)
     return simple<__half>(ctx, *cache, q, n_heads, tokens, lens, counts, out);
   return simple<__nv_bfloat16>(ctx, *cache, q, n_heads, tokens, lens, counts, out);

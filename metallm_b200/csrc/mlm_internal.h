@@ -41,6 +41,11 @@ struct mlm_ctx {
   size_t attn_partials_floats = 0;
   int *attn_arrivals = nullptr;  // per (sequence, KV head); zero between launches
 
+  // attention over the 4-bit cache: the CTAs' partial sums, and one arrival
+  // counter per CTA, zero between launches
+  float *kv4_parts = nullptr;
+  int *kv4_arrivals = nullptr;
+
   // stream-K hand-off flags of the prefill GEMM, one per output tile; zero
   // between launches (each launch's waiters count them back down)
   int *gemm_flags = nullptr;
