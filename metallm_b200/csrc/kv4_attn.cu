@@ -7,6 +7,7 @@
 // Pointers to data that earlier kernels write carry no __restrict__, so that no
 // load of it moves above the dependent wait.
 #include <algorithm>
+#include <type_traits>
 
 #include "mlm_device.cuh"
 #include "mlm_internal.h"
@@ -54,6 +55,16 @@ constexpr int kHalfStage = kBlk * kRow;      // K or V of a block
 constexpr int kStage = 2 * kHalfStage;
 constexpr int kPieceRow = kD + 2;            // a column of a piece: o[128], m, l
 constexpr int kMaxCols = 16;
+
+// a product from zero accumulators
+__device__ __forceinline__ void mma_f16_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                             uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 
 struct FewArgs {
   const uint8_t *kc, *vc;
@@ -109,6 +120,20 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
                : "memory");
   return v;
 }
+__device__ __forceinline__ void ldsm2_t(uint32_t addr, uint32_t (&r)[2]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
+               : "=r"(r[0]), "=r"(r[1])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t lds4(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float low_f16(uint32_t v) {
+  return __half2float(__ushort_as_half((unsigned short)v));
+}
 // the transpose of an 8x8 matrix of 16-bit elements, row r of it in lanes 4r ..
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
@@ -130,13 +155,20 @@ __device__ __forceinline__ uint32_t u4_get(const uint4 &v, int i) {
 // a position on the line of blocks
 struct Cursor {
   int b, h, blk, nb;  // block blk of nb of (b, h)
+  int len, count;     // of sequence b
 };
 
 template <int NT, bool DUP, int W, int STAGES, class OutT>
 __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
+  static_assert(2 * W <= 32, "a lane per piece");
   static_assert(!DUP || NT == 1, "hi and lo share one tile of columns");
   constexpr int kCols = DUP ? 4 : 8 * NT;
   constexpr int kPiece = kCols * kPieceRow;
+  // An fp16 output takes the weights as hi + lo (rounded to fp16 alone they would
+  // add as much error as the output's own rounding, as codes are not centred);
+  // for a bf16 output, eight times coarser, hi alone
+  constexpr bool LO = std::is_same<OutT, __half>::value;
+  constexpr bool kSplit = DUP && LO;  // columns 4 .. 7 hold the lo parts
   static_assert(kPiece * 4 <= STAGES * kStage, "a warp's last piece lies in its ring");
   extern __shared__ __align__(128) uint8_t smem[];
   // rings, the warps' head pieces, the line's offsets per sequence
@@ -194,7 +226,9 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
   const int quota = max(W, (total + (int)gridDim.x - 1) / (int)gridDim.x);
   const int cta0 = min(total, (int)blockIdx.x * quota), cta1 = min(total, cta0 + quota);
   if (cta0 >= cta1) return;
-  const int w0 = cta0 + (cta1 - cta0) * warp / W, w1 = cta0 + (cta1 - cta0) * (warp + 1) / W;
+  // the warps with blocks are the first ones
+  const int per = (cta1 - cta0) / W, more = (cta1 - cta0) % W;
+  const int w0 = cta0 + warp * per + min(warp, more), w1 = w0 + per + (warp < more ? 1 : 0);
 
   auto at = [&](int x) {
     int lo = 0, hi = a.batch;  // the last b with s_off[b] <= x
@@ -204,7 +238,8 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
     }
     Cursor c;
     c.b = lo;
-    c.nb = (s_off[lo + 1] - s_off[lo]) / a.n_kv;
+    seq_shape(a.lens, a.counts, lo, a.tokens, a.capacity, c.len, c.count);
+    c.nb = (c.len + kBlk - 1) / kBlk;
     const int rem = x - s_off[lo];
     c.h = rem / c.nb;
     c.blk = rem - c.h * c.nb;
@@ -216,43 +251,74 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
     if (++c.h < a.n_kv) return;
     c.h = 0;
     do ++c.b; while (c.b < a.batch && s_off[c.b + 1] == s_off[c.b]);
-    if (c.b < a.batch) c.nb = (s_off[c.b + 1] - s_off[c.b]) / a.n_kv;
+    if (c.b == a.batch) return;
+    seq_shape(a.lens, a.counts, c.b, a.tokens, a.capacity, c.len, c.count);
+    c.nb = (c.len + kBlk - 1) / kBlk;
   };
-  auto issue = [&](const Cursor &c, int stage) {  // one lane
-    int len, count;
-    seq_shape(a.lens, a.counts, c.b, a.tokens, a.capacity, len, count);
-    const uint32_t bytes = (uint32_t)min(kBlk, len - c.blk * kBlk) * kRow;
-    const size_t off = (((size_t)c.b * a.n_kv + c.h) * a.capacity + (size_t)c.blk * kBlk) * kRow;
-    const uint32_t bar = bar0 + 8 * stage, dst = ring + stage * kStage;
-    mbar_expect_tx(bar, 2 * bytes);
-    bulk_copy(dst, a.kc + off, bytes, bar);
-    bulk_copy(dst + kHalfStage, a.vc + off, bytes, bar);
+  const long long k_to_v = a.vc - a.kc;
+  const uint8_t *src = nullptr;  // the next block to copy
+  auto source = [&](const Cursor &c) {
+    return a.kc + (((size_t)c.b * a.n_kv + c.h) * a.capacity + (size_t)c.blk * kBlk) * kRow;
+  };
+  // copy block `ahead` into a stage and move on
+  auto issue = [&](Cursor &c, int stage) {
+    if (lane == 0) {
+      const uint32_t bytes = (uint32_t)min(kBlk, c.len - c.blk * kBlk) * kRow;
+      const uint32_t bar = bar0 + 8 * stage, dst = ring + stage * kStage;
+      mbar_expect_tx(bar, 2 * bytes);
+      bulk_copy(dst, src, bytes, bar);
+      bulk_copy(dst + kHalfStage, src + k_to_v, bytes, bar);
+    }
+    next(c);
+    if (c.blk)
+      src += kHalfStage;
+    else if (c.b < a.batch)
+      src = source(c);
   };
 
   Cursor cur = {}, ahead = {};
   int issued = w0;
   if (w0 < w1) {
     cur = ahead = at(w0);
-    for (; issued < min(w1, w0 + STAGES); ++issued) {
-      if (lane == 0) issue(ahead, issued - w0);
-      next(ahead);
-    }
+    src = source(ahead);
+    for (; issued < min(w1, w0 + STAGES); ++issued) issue(ahead, issued - w0);
   }
+
+  // B operands of the V product: the weights as fp16, hi and lo where both are
+  // wanted; with shared columns a lane's b is one or the other
+  const float part = kSplit && r >= 4 ? 1.f : 0.f;
+  auto split = [&](float v0, float v1, float v2, float v3, uint32_t &b0, uint32_t &b1, uint32_t &l0,
+                   uint32_t &l1) {
+    b0 = pack_f16(v0, v1);
+    b1 = pack_f16(v2, v3);
+    l0 = l1 = 0;
+    if (!LO) return;
+    const float2 h0 = unpack_f16(b0), h1 = unpack_f16(b1);
+    if (DUP) {
+      b0 = pack_f16(fmaf(-part, h0.x, v0), fmaf(-part, h0.y, v1));
+      b1 = pack_f16(fmaf(-part, h1.x, v2), fmaf(-part, h1.y, v3));
+    } else {
+      l0 = pack_f16(v0 - h0.x, v1 - h0.y);
+      l1 = pack_f16(v2 - h1.x, v3 - h1.y);
+    }
+  };
 
   // queries: the B operand of K's products, per group of 32 dimensions
   uint32_t qb[NT][4][4];
-  float qs[NT][4][2];          // sums of the scaled q over a group, columns 2 t4, 2 t4 + 1
   float cs[NT];                // score scale of column r, in powers of two
   int seen[NT];                // rows column r attends to
-  int len = 0, count = 0, seen_min = 0;
-  float o[NT][4][2][4], om[NT][4], mx[NT], l[NT];
+  uint32_t qm[NT][2];          // the B operand of K's minima: (0, group sum) per group, hi and lo
+  int seen_min = 0;
+  float o[NT][4][2][4], mx[NT], l[NT];
+  float om[NT][4];             // sum of p m: rows 2 g + 1 of the product with V's scales
+  float omf[NT][4];            // the same of masked blocks, group g, this lane's rows
   bool ok = true;
   int first = w0;              // where the current item starts within this warp's stretch
 
   for (int x = w0; x < w1; ++x) {
     if (x == w0 || cur.blk == 0) {
       first = x;
-      seq_shape(a.lens, a.counts, cur.b, a.tokens, a.capacity, len, count);
+      const int len = cur.len, count = cur.count;
       seen_min = max(0, len - count + 1);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -294,10 +360,13 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
           qb[nt][g][3] = pack_f16(f[g][3] * 0.0625f, f[g][7] * 0.0625f);
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          sum *= 5.9604644775390625e-08f;  // 2^-24, the codes' unit
-          qs[nt][g][0] = __shfl_sync(0xffffffffu, sum, 8 * t4);
-          qs[nt][g][1] = __shfl_sync(0xffffffffu, sum, 8 * t4 + 4);
-          om[nt][g] = 0.f;
+          sum *= 0.015625f;  // at most 32 x 2^14: below 2^13
+          const float hi = __half2float(__float2half_rn(sum));
+          if (t4 == g) {
+            qm[nt][0] = pack_f16(0.f, hi);
+            qm[nt][1] = pack_f16(0.f, sum - hi);
+          }
+          om[nt][g] = omf[nt][g] = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[nt][g][0][i] = o[nt][g][1][i] = 0.f;
         }
@@ -313,147 +382,174 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
       break;
     }
 
-    // scores of the block's two 16-row tiles
-    const uint32_t tile_lane = (uint32_t)((((lane >> 3) & 1) * 8 + (lane & 7)) * kRow + (lane >> 4) * 16);
-    float sT[NT][2][2][2];  // column r: rows 16 kt + 8 half + 2 t4 + {0, 1}
+    const bool masked = (cur.blk + 1) * kBlk > seen_min;  // uniform in the warp
+    auto block = [&](auto mask_tag) {
+      constexpr bool MASK = decltype(mask_tag)::value;
+      const uint32_t tile_lane =
+          (uint32_t)((((lane >> 3) & 1) * 8 + (lane & 7)) * kRow + (lane >> 4) * 16);
+      // scores of the block's two 16-row tiles
+      float sT[NT][2][2][2];  // column r: rows 16 kt + 8 half + 2 t4 + {0, 1}
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      uint32_t w[2][4];
-      ldsm4(sk + kt * 16 * kRow + tile_lane, w[0]);
-      ldsm4(sk + kt * 16 * kRow + tile_lane + 32, w[1]);
-      const uint4 dm0 = lds16(sk + (kt * 16 + r) * kRow + 64);
-      const uint4 dm1 = lds16(sk + (kt * 16 + r + 8) * kRow + 64);
-      float s[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const uint32_t wa = w[g >> 1][(g & 1) * 2], wb = w[g >> 1][(g & 1) * 2 + 1];
-        const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
-        const float2 f0 = unpack_f16(u4_get(dm0, g)), f1 = unpack_f16(u4_get(dm1, g));
+      for (int kt = 0; kt < 2; ++kt) {
+        uint32_t w[2][4];
+        ldsm4(sk + kt * 16 * kRow + tile_lane, w[0]);
+        ldsm4(sk + kt * 16 * kRow + tile_lane + 32, w[1]);
+        const uint4 dm0 = lds16(sk + (kt * 16 + r) * kRow + 64);
+        const uint4 dm1 = lds16(sk + (kt * 16 + r + 8) * kRow + 64);
+        // sum_g m_g (sum q): the scale words (d, m) are an A operand already
+        const uint32_t me0 = lds4(sk + (kt * 16 + r) * kRow + 64 + 4 * t4);
+        const uint32_t me1 = lds4(sk + (kt * 16 + r + 8) * kRow + 64 + 4 * t4);
+        float s[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_f16_16816(acc, wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u,
-                        wb & 0x00F000F0u, qb[nt][g][0], qb[nt][g][1]);
-          mma_f16_16816(acc, wa8 & 0x000F000Fu, wb8 & 0x000F000Fu, wa8 & 0x00F000F0u,
-                        wb8 & 0x00F000F0u, qb[nt][g][2], qb[nt][g][3]);
-          s[nt][0] = fmaf(f0.x, acc[0], fmaf(f0.y, qs[nt][g][0], s[nt][0]));
-          s[nt][1] = fmaf(f0.x, acc[1], fmaf(f0.y, qs[nt][g][1], s[nt][1]));
-          s[nt][2] = fmaf(f1.x, acc[2], fmaf(f1.y, qs[nt][g][0], s[nt][2]));
-          s[nt][3] = fmaf(f1.x, acc[3], fmaf(f1.y, qs[nt][g][1], s[nt][3]));
+          float acc[4];
+          mma_f16_zero(acc, me0, me1, me0, me1, qm[nt][0], qm[nt][1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[nt][i] = acc[i] * 3.814697265625e-06f;  // to units of 2^-24
         }
-      }
-      // rows x columns to columns x rows, as the V product's B operand wants
-      // the weights: 32-bit values as two 16-bit matrices
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t v0 = __float_as_uint(s[nt][2 * half]), v1 = __float_as_uint(s[nt][2 * half + 1]);
-          const uint32_t lo = transpose8(__byte_perm(v0, v1, 0x5410));
-          const uint32_t hi = transpose8(__byte_perm(v0, v1, 0x7632));
-          sT[nt][kt][half][0] = cs[nt] * __uint_as_float(__byte_perm(lo, hi, 0x5410));
-          sT[nt][kt][half][1] = cs[nt] * __uint_as_float(__byte_perm(lo, hi, 0x7632));
-        }
-    }
-    const int row0 = cur.blk * kBlk + 2 * t4;  // this lane's first row of the block
-    const bool masked = (cur.blk + 1) * kBlk > seen_min;  // uniform in the warp
-    if (masked) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (row0 + (i >> 2) * 16 + ((i >> 1) & 1) * 8 + (i & 1) >= seen[nt])
-            sT[nt][i >> 2][(i >> 1) & 1][i & 1] = -INFINITY;
-    }
-    // running maximum and sum; the weights carry a factor of 4 (p <= 4), which
-    // l carries too: p d stays an fp16 value for every d below 2^14
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float top = mx[nt];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, sT[nt][i >> 2][(i >> 1) & 1][i & 1]);
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (__any_sync(0xffffffffu, top != mx[nt])) {
-        const float f = top == mx[nt] ? 1.f : ex2(mx[nt] - top);
-        l[nt] *= f;
-        const float f0 = __shfl_sync(0xffffffffu, f, 8 * t4), f1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          om[nt][g] *= f;
+          const uint32_t wa = w[g >> 1][(g & 1) * 2], wb = w[g >> 1][(g & 1) * 2 + 1];
+          const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
+          const float d0 = low_f16(u4_get(dm0, g)), d1 = low_f16(u4_get(dm1, g));
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            o[nt][g][i][0] *= f0;
-            o[nt][g][i][1] *= f1;
-            o[nt][g][i][2] *= f0;
-            o[nt][g][i][3] *= f1;
+          for (int nt = 0; nt < NT; ++nt) {
+            float acc[4];
+            mma_f16_zero(acc, wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u,
+                         wb & 0x00F000F0u, qb[nt][g][0], qb[nt][g][1]);
+            mma_f16_16816(acc, wa8 & 0x000F000Fu, wb8 & 0x000F000Fu, wa8 & 0x00F000F0u,
+                          wb8 & 0x00F000F0u, qb[nt][g][2], qb[nt][g][3]);
+            s[nt][0] = fmaf(d0, acc[0], s[nt][0]);
+            s[nt][1] = fmaf(d0, acc[1], s[nt][1]);
+            s[nt][2] = fmaf(d1, acc[2], s[nt][2]);
+            s[nt][3] = fmaf(d1, acc[3], s[nt][3]);
           }
         }
-        mx[nt] = top;
-      }
-      const float base = (top == -INFINITY ? 0.f : top) - 2.f;
+        // rows x columns to columns x rows, as the V product's B operand wants
+        // the weights: 32-bit values as two 16-bit matrices
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float &v = sT[nt][i >> 2][(i >> 1) & 1][i & 1];
-        v = ex2(v - base);
-        l[nt] += v;
-      }
-    }
-    // o += (p d) c and the m part
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      uint32_t w[2][4];
-      ldsm4_t(sv + kt * 16 * kRow + tile_lane, w[0]);
-      ldsm4_t(sv + kt * 16 * kRow + tile_lane + 32, w[1]);
-      uint4 dm[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        dm[i] = lds16(sv + (kt * 16 + (i >> 1) * 8 + 2 * t4 + (i & 1)) * kRow + 64);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const uint32_t wa = w[g >> 1][(g & 1) * 2], wb = w[g >> 1][(g & 1) * 2 + 1];
-        const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
-        float2 f[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = unpack_f16(u4_get(dm[i], g));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float v[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float p = sT[nt][kt][i >> 1][i & 1];
-            v[i] = p * f[i].x;
-            float pm = p * f[i].y;
-            // a row this column does not see adds nothing, whatever its scales hold
-            if (masked && row0 + kt * 16 + (i >> 1) * 8 + (i & 1) >= seen[nt]) v[i] = pm = 0.f;
-            om[nt][g] += pm;
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t v0 = __float_as_uint(s[nt][2 * half]),
+                           v1 = __float_as_uint(s[nt][2 * half + 1]);
+            const uint32_t lo = transpose8(__byte_perm(v0, v1, 0x5410));
+            const uint32_t hi = transpose8(__byte_perm(v0, v1, 0x7632));
+            sT[nt][kt][half][0] = __uint_as_float(__byte_perm(lo, hi, 0x5410));
+            sT[nt][kt][half][1] = __uint_as_float(__byte_perm(lo, hi, 0x7632));
           }
-          uint32_t b0 = pack_f16(v[0], v[1]), b1 = pack_f16(v[2], v[3]);
-          const float2 h0 = unpack_f16(b0), h1 = unpack_f16(b1);
-          const uint32_t l0 = pack_f16(v[0] - h0.x, v[1] - h0.y), l1 = pack_f16(v[2] - h1.x, v[3] - h1.y);
-          if (DUP && r >= 4) {
-            b0 = l0;
-            b1 = l1;
+      }
+      const int row0 = cur.blk * kBlk + 2 * t4;  // this lane's first row of the block
+      if (MASK) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (row0 + (i >> 2) * 16 + ((i >> 1) & 1) * 8 + (i & 1) >= seen[nt])
+              sT[nt][i >> 2][(i >> 1) & 1][i & 1] = -INFINITY;
+      }
+      // running maximum and sum; the weights carry a factor of 4 (p <= 4), which
+      // l carries too: p d stays an fp16 value for every d below 2^14
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float top = mx[nt];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, sT[nt][i >> 2][(i >> 1) & 1][i & 1]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (__any_sync(0xffffffffu, top != mx[nt])) {
+          const float f = top == mx[nt] ? 1.f : ex2((mx[nt] - top) * cs[nt]);
+          l[nt] *= f;
+          const float f0 = __shfl_sync(0xffffffffu, f, 8 * t4),
+                      f1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            omf[nt][g] *= f;
+            om[nt][g] *= (g & 1) ? f1 : f0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              o[nt][g][i][0] *= f0;
+              o[nt][g][i][1] *= f1;
+              o[nt][g][i][2] *= f0;
+              o[nt][g][i][3] *= f1;
+            }
           }
-          mma_f16_16816(o[nt][g][0], wa & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x000F000Fu,
-                        wb & 0x00F000F0u, b0, b1);
-          mma_f16_16816(o[nt][g][1], wa8 & 0x000F000Fu, wa8 & 0x00F000F0u, wb8 & 0x000F000Fu,
-                        wb8 & 0x00F000F0u, b0, b1);
-          if (!DUP) {
+          mx[nt] = top;
+        }
+        const float base = fmaf(top == -INFINITY ? 0.f : top, -cs[nt], 2.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float &v = sT[nt][i >> 2][(i >> 1) & 1][i & 1];
+          v = ex2(fmaf(v, cs[nt], base));
+          l[nt] += v;
+        }
+      }
+      // o += (p d) c and the m part
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        uint32_t w[2][4];
+        ldsm4_t(sv + kt * 16 * kRow + tile_lane, w[0]);
+        ldsm4_t(sv + kt * 16 * kRow + tile_lane + 32, w[1]);
+        uint4 dm[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          dm[i] = lds16(sv + (kt * 16 + (i >> 1) * 8 + 2 * t4 + (i & 1)) * kRow + 64);
+        if (!MASK) {
+          // sum_j p_j m_jg (and p_j d_jg, unused): the transposed scale words
+          uint32_t mt[2];
+          ldsm2_t(sv + (kt * 16 + (lane & 15)) * kRow + 64, mt);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float(&p)[2][2] = sT[nt][kt];
+            uint32_t b0, b1, l0, l1;
+            split(p[0][0], p[0][1], p[1][0], p[1][1], b0, b1, l0, l1);
+            mma_f16_16816(om[nt], mt[0], 0u, mt[1], 0u, b0, b1);
+            if (LO && !DUP) mma_f16_16816(om[nt], mt[0], 0u, mt[1], 0u, l0, l1);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const uint32_t wa = w[g >> 1][(g & 1) * 2], wb = w[g >> 1][(g & 1) * 2 + 1];
+          const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = sT[nt][kt][i >> 1][i & 1];
+              if (MASK) {
+                // a row this column does not see adds nothing, whatever its scales hold
+                const float2 f = unpack_f16(u4_get(dm[i], g));
+                const bool sees = row0 + kt * 16 + (i >> 1) * 8 + (i & 1) < seen[nt];
+                v[i] = sees ? p * f.x : 0.f;
+                omf[nt][g] += sees ? p * f.y : 0.f;
+              } else {
+                v[i] = p * low_f16(u4_get(dm[i], g));
+              }
+            }
+            uint32_t b0, b1, l0, l1;
+            split(v[0], v[1], v[2], v[3], b0, b1, l0, l1);
             mma_f16_16816(o[nt][g][0], wa & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x000F000Fu,
-                          wb & 0x00F000F0u, l0, l1);
+                          wb & 0x00F000F0u, b0, b1);
             mma_f16_16816(o[nt][g][1], wa8 & 0x000F000Fu, wa8 & 0x00F000F0u, wb8 & 0x000F000Fu,
-                          wb8 & 0x00F000F0u, l0, l1);
+                          wb8 & 0x00F000F0u, b0, b1);
+            if (LO && !DUP) {
+              mma_f16_16816(o[nt][g][0], wa & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x000F000Fu,
+                            wb & 0x00F000F0u, l0, l1);
+              mma_f16_16816(o[nt][g][1], wa8 & 0x000F000Fu, wa8 & 0x00F000F0u,
+                            wb8 & 0x000F000Fu, wb8 & 0x00F000F0u, l0, l1);
+            }
           }
         }
       }
-    }
+    };
+    if (masked)
+      block(std::true_type());
+    else
+      block(std::false_type());
     __syncwarp();  // every lane is done with the stage
     if (issued < w1) {
-      if (lane == 0) issue(ahead, stage);
-      next(ahead);
+      issue(ahead, stage);
       ++issued;
     }
 
@@ -467,23 +563,31 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
                                  : s_head + warp * kPiece;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        const int count = cur.count;
         l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], 1);
         l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], 2);
         const float inv = whole ? (l[nt] > 0.f ? 1.f / l[nt] : (l[nt] == 0.f ? 0.f : NAN)) : 1.f;
         const float i0 = __shfl_sync(0xffffffffu, inv, 8 * t4), i1 = __shfl_sync(0xffffffffu, inv, 8 * t4 + 4);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          float m = om[nt][g];
+          float m = omf[nt][g];
           m += __shfl_xor_sync(0xffffffffu, m, 1);
           m += __shfl_xor_sync(0xffffffffu, m, 2);
-          const float m0 = __shfl_sync(0xffffffffu, m, 8 * t4), m1 = __shfl_sync(0xffffffffu, m, 8 * t4 + 4);
+          float m0 = __shfl_sync(0xffffffffu, om[nt][0], 4 * (2 * g + 1) + t4),
+                m1 = __shfl_sync(0xffffffffu, om[nt][1], 4 * (2 * g + 1) + t4);
+          if (kSplit) {
+            m0 += __shfl_xor_sync(0xffffffffu, m0, 2);
+            m1 += __shfl_xor_sync(0xffffffffu, m1, 2);
+          }
+          m0 += __shfl_sync(0xffffffffu, m, 8 * t4);
+          m1 += __shfl_sync(0xffffffffu, m, 8 * t4 + 4);
           float v[2][4];  // columns 2 t4 and 2 t4 + 1, dimensions 32 g + 4 r ..
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               float w = o[nt][g][i][c];
-              if (DUP) w += __shfl_xor_sync(0xffffffffu, w, 2);  // hi + lo
+              if (kSplit) w += __shfl_xor_sync(0xffffffffu, w, 2);  // hi + lo
               // the codes' unit: 2^-24, and 16 times that in rows 8 .. 15
               v[c & 1][2 * i + (c >> 1)] = fmaf(w, c < 2 ? 16777216.f : 1048576.f, (c & 1) ? m1 : m0);
             }
@@ -511,7 +615,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
           }
         }
         if (!whole && t4 == 0 && (!DUP || r < 4)) {
-          piece[(nt * 8 + r) * kPieceRow + kD] = mx[nt];
+          piece[(nt * 8 + r) * kPieceRow + kD] = mx[nt] * cs[nt];
           piece[(nt * 8 + r) * kPieceRow + kD + 1] = l[nt];
         }
       }
@@ -527,89 +631,92 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
       mbar_wait_bounded(bar0 + 8 * s, (uint32_t)((issued - w0 - 1 - s) / STAGES) & 1, a.status);
   __syncthreads();
 
-  // join the pieces: a run of slots holding one item at a time
-  auto piece_of = [&](int slot) -> const float * {
-    return (slot & 1) ? reinterpret_cast<const float *>(smem + (slot >> 1) * STAGES * kStage)
-                      : s_head + (slot >> 1) * kPiece;
-  };
-  auto emit = [&](int bh, int col, int d, float v) {
-    const int b = bh / a.n_kv, h = bh - b * a.n_kv;
-    int n, c;
-    seq_shape(a.lens, a.counts, b, a.tokens, a.capacity, n, c);
-    if (col >= c * a.group) return;
-    const int tok = col / a.group;
-    reinterpret_cast<OutT *>(a.out)[(((size_t)b * a.tokens + tok) * a.n_heads + h * a.group +
-                                     (col - tok * a.group)) * kD + d] = from_float<OutT>(v);
-  };
-  for (int s0 = 0; s0 < 2 * W;) {
-    const int item = s_item[s0];
-    if (item < 0) {
-      ++s0;
-      continue;
-    }
-    int s1 = s0 + 1;
-    while (s1 < 2 * W && (s_item[s1] < 0 || s_item[s1] == item)) ++s1;
-    const int bh = s_bh[s0], b = bh / a.n_kv;
+  // Join the pieces.  A slot per lane; an item's pieces are one per warp of a
+  // range of warps: in the ring where the warp's stretch ended inside the item, its
+  // head slot where the item ended first.
+  const int my_item = lane < 2 * W ? s_item[lane] : -1;
+  uint32_t left = __ballot_sync(0xffffffffu, my_item >= 0);
+  while (left) {
+    const int s0 = __ffs(left) - 1;
+    const int item = __shfl_sync(0xffffffffu, my_item, s0);
+    const uint32_t group = __ballot_sync(0xffffffffu, my_item == item) & left;
+    left &= ~group;
+    const int s1 = 31 - __clz(group);
+    const int first_warp = s0 >> 1, n = (s1 >> 1) - first_warp + 1;
+    const int bh = s_bh[s0], b = bh / a.n_kv, h = bh - b * a.n_kv;
     const int nb = (s_off[b + 1] - s_off[b]) / a.n_kv;
     const bool complete = item >= cta0 && item + nb <= cta1;
-    float *part = a.parts + ((size_t)blockIdx.x * 2 + (item < cta0 ? 0 : 1)) * kMaxCols * kPieceRow;
-    for (int i = threadIdx.x; i < kCols * kD; i += W * 32) {
-      const int col = i / kD, d = i - col * kD;
-      float top = -INFINITY;
-      for (int s = s0; s < s1; ++s)
-        if (s_item[s] >= 0) top = fmaxf(top, piece_of(s)[col * kPieceRow + kD]);
-      float sum = 0.f, v = 0.f;
-      for (int s = s0; s < s1; ++s) {
-        if (s_item[s] < 0) continue;
-        const float *p = piece_of(s) + col * kPieceRow;
-        const float f = p[kD] == top ? 1.f : ex2(p[kD] - top);
-        v += f * p[d];
-        sum += f * p[kD + 1];
-      }
+    int len, count;
+    seq_shape(a.lens, a.counts, b, a.tokens, a.capacity, len, count);
+    auto piece_of = [&](int i) -> const float * {  // of warp first_warp + i
+      return i == n - 1 && !(s1 & 1)
+                 ? s_head + (first_warp + i) * kPiece
+                 : reinterpret_cast<const float *>(smem + (first_warp + i) * STAGES * kStage);
+    };
+    auto emit = [&](int col, int d, float v) {
+      if (col >= count * a.group) return;
+      const int tok = col / a.group;
+      reinterpret_cast<OutT *>(a.out)[(((size_t)b * a.tokens + tok) * a.n_heads + h * a.group +
+                                       (col - tok * a.group)) * kD + d] = from_float<OutT>(v);
+    };
+    float *mine = a.parts + ((size_t)blockIdx.x * 2 + (item < cta0 ? 0 : 1)) * kMaxCols * kPieceRow;
+    // a warp takes 32 dimensions of a column; lane i holds piece i's statistics
+    for (int i = warp; i < kCols * kD / 32; i += W) {
+      const int col = i / (kD / 32), d = i % (kD / 32) * 32 + lane;
+      const float *pm = piece_of(min(lane, n - 1)) + col * kPieceRow;
+      const float m = lane < n ? pm[kD] : -INFINITY;
+      const float top = warp_max(m);
+      const float f = m == top ? 1.f : ex2(m - top);
+      const float sum = warp_sum(lane < n ? f * pm[kD + 1] : 0.f);
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < W; ++k)
+        if (k < n) v = fmaf(__shfl_sync(0xffffffffu, f, k), piece_of(k)[col * kPieceRow + d], v);
       if (complete) {
-        emit(bh, col, d, sum == 0.f ? 0.f : v / sum);
+        emit(col, d, sum == 0.f ? 0.f : v / sum);
       } else {
-        part[col * kPieceRow + d] = v;
+        mine[col * kPieceRow + d] = v;
         if (d == 0) {
-          part[col * kPieceRow + kD] = top;
-          part[col * kPieceRow + kD + 1] = sum;
+          mine[col * kPieceRow + kD] = top;
+          mine[col * kPieceRow + kD + 1] = sum;
         }
       }
     }
-    if (!complete) {
-      // the last CTA of the item to arrive joins the CTAs' parts, in order
-      const int c0 = item / quota, c1 = (item + nb - 1) / quota;
+    if (complete) continue;
+    // the last CTA of the item to arrive joins the CTAs' parts, in order
+    const int c0 = item / quota, c1 = (item + nb - 1) / quota;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      s_last = atomicAdd(a.arrivals + c0, 1) == c1 - c0;
+      if (s_last) a.arrivals[c0] = 0;
+    }
+    __syncthreads();
+    if (s_last) {
       __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        const int n = atomicAdd(a.arrivals + c0, 1);
-        s_last = n == c1 - c0;
-        if (s_last) a.arrivals[c0] = 0;
-      }
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        for (int i = threadIdx.x; i < kCols * kD; i += W * 32) {
-          const int col = i / kD, d = i - col * kD;
-          auto of = [&](int c) {
-            return a.parts + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kMaxCols * kPieceRow + col * kPieceRow;
-          };
-          float top = -INFINITY;
-          for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(of(c) + kD));
-          float sum = 0.f, v = 0.f;
-#pragma unroll 4
-          for (int c = c0; c <= c1; ++c) {
-            const float m = __ldcg(of(c) + kD);
-            const float f = m == top ? 1.f : ex2(m - top);
-            v += f * __ldcg(of(c) + d);
-            sum += f * __ldcg(of(c) + kD + 1);
-          }
-          emit(bh, col, d, sum == 0.f ? 0.f : v / sum);
+      for (int i = warp; i < kCols * kD / 32; i += W) {
+        const int col = i / (kD / 32), d = i % (kD / 32) * 32 + lane;
+        auto part_of = [&](int c) {
+          return a.parts + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kMaxCols * kPieceRow + col * kPieceRow;
+        };
+        float top = -INFINITY;
+        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(part_of(c) + kD));
+        top = warp_max(top);
+        float v = 0.f, sum = 0.f;
+        for (int cb = c0; cb <= c1; cb += 32) {
+          const int c = min(cb + lane, c1), k1 = min(32, c1 - cb + 1);
+          const float m = __ldcg(part_of(c) + kD);
+          const float f = cb + lane > c1 ? 0.f : m == top ? 1.f : ex2(m - top);
+          sum += cb + lane > c1 ? 0.f : f * __ldcg(part_of(c) + kD + 1);
+#pragma unroll 8
+          for (int k = 0; k < k1; ++k)
+            v = fmaf(__shfl_sync(0xffffffffu, f, k), __ldcg(part_of(cb + k) + d), v);
         }
+        sum = warp_sum(sum);
+        emit(col, d, sum == 0.f ? 0.f : v / sum);
       }
-      __syncthreads();
     }
-    s0 = s1;
+    __syncthreads();
   }
 }
 
