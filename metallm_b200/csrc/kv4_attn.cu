@@ -152,10 +152,10 @@ __device__ __forceinline__ uint32_t u4_get(const uint4 &v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
-// a position on the line of blocks
-struct Cursor {
-  int b, h, blk, nb;  // block blk of nb of (b, h)
-  int len, count;     // of sequence b
+// an item (the blocks of one KV head of one sequence) and a block of it
+struct Item {
+  int b, h, blk, nb;
+  int len, count;  // of sequence b
 };
 
 template <int NT, bool DUP, int W, int STAGES, class OutT>
@@ -222,11 +222,11 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
     OutT *o = reinterpret_cast<OutT *>(a.out) + (size_t)b * a.tokens * a.n_heads * kD;
     for (int i = threadIdx.x; i < count * a.n_heads * kD; i += W * 32) o[i] = from_float<OutT>(0.f);
   }
-  // equal stretches, at least one block per warp
-  const int quota = max(W, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  // equal stretches; a CTA with few blocks gives them to its first warps, one
+  // per SM quarter
+  const int quota = max(4, (total + (int)gridDim.x - 1) / (int)gridDim.x);
   const int cta0 = min(total, (int)blockIdx.x * quota), cta1 = min(total, cta0 + quota);
   if (cta0 >= cta1) return;
-  // the warps with blocks are the first ones
   const int per = (cta1 - cta0) / W, more = (cta1 - cta0) % W;
   const int w0 = cta0 + warp * per + min(warp, more), w1 = w0 + per + (warp < more ? 1 : 0);
 
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
       const int mid = (lo + hi) >> 1;
       if (s_off[mid] <= x) lo = mid; else hi = mid;
     }
-    Cursor c;
+    Item c;
     c.b = lo;
     seq_shape(a.lens, a.counts, lo, a.tokens, a.capacity, c.len, c.count);
     c.nb = (c.len + kBlk - 1) / kBlk;
@@ -245,8 +245,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
     c.blk = rem - c.h * c.nb;
     return c;
   };
-  auto next = [&](Cursor &c) {
-    if (++c.blk < c.nb) return;
+  auto next_item = [&](Item &c) {
     c.blk = 0;
     if (++c.h < a.n_kv) return;
     c.h = 0;
@@ -255,34 +254,36 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
     seq_shape(a.lens, a.counts, c.b, a.tokens, a.capacity, c.len, c.count);
     c.nb = (c.len + kBlk - 1) / kBlk;
   };
-  const long long k_to_v = a.vc - a.kc;
-  const uint8_t *src = nullptr;  // the next block to copy
-  auto source = [&](const Cursor &c) {
+  auto source = [&](const Item &c) {
     return a.kc + (((size_t)c.b * a.n_kv + c.h) * a.capacity + (size_t)c.blk * kBlk) * kRow;
   };
-  // copy block `ahead` into a stage and move on
-  auto issue = [&](Cursor &c, int stage) {
+  Item cur = {}, ahead = {};
+  const uint8_t *src = nullptr;  // the next block to copy
+  const long long k_to_v = a.vc - a.kc;
+  int to_copy = w1 - w0;
+  if (to_copy > 0) {
+    cur = ahead = at(w0);
+    src = source(ahead);
+  }
+  // copy the next block into a stage and move on
+  auto copy = [&](int stage) {
     if (lane == 0) {
-      const uint32_t bytes = (uint32_t)min(kBlk, c.len - c.blk * kBlk) * kRow;
+      const uint32_t bytes = (uint32_t)min(kBlk, ahead.len - ahead.blk * kBlk) * kRow;
       const uint32_t bar = bar0 + 8 * stage, dst = ring + stage * kStage;
       mbar_expect_tx(bar, 2 * bytes);
       bulk_copy(dst, src, bytes, bar);
       bulk_copy(dst + kHalfStage, src + k_to_v, bytes, bar);
     }
-    next(c);
-    if (c.blk)
-      src += kHalfStage;
-    else if (c.b < a.batch)
-      src = source(c);
+    --to_copy;
+    src += kHalfStage;
+    if (++ahead.blk == ahead.nb && to_copy > 0) {
+      next_item(ahead);
+      src = source(ahead);
+    }
   };
-
-  Cursor cur = {}, ahead = {};
-  int issued = w0;
-  if (w0 < w1) {
-    cur = ahead = at(w0);
-    src = source(ahead);
-    for (; issued < min(w1, w0 + STAGES); ++issued) issue(ahead, issued - w0);
-  }
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i)
+    if (to_copy > 0) copy(i);
 
   // B operands of the V product: the weights as fp16, hi and lo where both are
   // wanted; with shared columns a lane's b is one or the other
@@ -308,18 +309,22 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
   float cs[NT];                // score scale of column r, in powers of two
   int seen[NT];                // rows column r attends to
   uint32_t qm[NT][2];          // the B operand of K's minima: (0, group sum) per group, hi and lo
-  int seen_min = 0;
   float o[NT][4][2][4], mx[NT], l[NT];
   float om[NT][4];             // sum of p m: rows 2 g + 1 of the product with V's scales
   float omf[NT][4];            // the same of masked blocks, group g, this lane's rows
+  float slack[NT];             // a score's lead over the maximum that is let pass
   bool ok = true;
-  int first = w0;              // where the current item starts within this warp's stretch
+  int stage = 0;
+  uint32_t phase = 0;
 
-  for (int x = w0; x < w1; ++x) {
-    if (x == w0 || cur.blk == 0) {
-      first = x;
+  for (int x = w0; x < w1;) {
+    const int first_blk = cur.blk;
+    const int end_blk = min(cur.nb, cur.blk + w1 - x);  // this stretch's part of the item
+    x += end_blk - first_blk;
+    int mask_from;  // the first block with a row that some token does not see
+    {
       const int len = cur.len, count = cur.count;
-      seen_min = max(0, len - count + 1);
+      mask_from = max(0, len - count + 1) / kBlk;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int col = DUP ? (r & 3) : nt * 8 + r;
@@ -346,6 +351,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
         const int e = big > 0.f ? 13 - ((int)((__float_as_uint(big) >> 23) & 0xFF) - 127) : 0;
         const float up = __uint_as_float((uint32_t)(e + 127) << 23);
         cs[nt] = kInvSqrtD * kLog2e * __uint_as_float((uint32_t)(24 - e + 127) << 23);
+        slack[nt] = 8.f / cs[nt];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           float sum = 0.f;
@@ -374,17 +380,9 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
         l[nt] = 0.f;
       }
     }
-    const int stage = (x - w0) % STAGES;
-    const uint32_t sk = ring + stage * kStage, sv = sk + kHalfStage;
-    ok = mbar_wait_bounded(bar0 + 8 * stage, (uint32_t)((x - w0) / STAGES) & 1, a.status);
-    if (!__all_sync(0xffffffffu, ok)) {
-      ok = false;
-      break;
-    }
-
-    const bool masked = (cur.blk + 1) * kBlk > seen_min;  // uniform in the warp
     auto block = [&](auto mask_tag) {
       constexpr bool MASK = decltype(mask_tag)::value;
+      const uint32_t sk = ring + stage * kStage, sv = sk + kHalfStage;
       const uint32_t tile_lane =
           (uint32_t)((((lane >> 3) & 1) * 8 + (lane & 7)) * kRow + (lane >> 4) * 16);
       // scores of the block's two 16-row tiles
@@ -448,16 +446,18 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
             if (row0 + (i >> 2) * 16 + ((i >> 1) & 1) * 8 + (i & 1) >= seen[nt])
               sT[nt][i >> 2][(i >> 1) & 1][i & 1] = -INFINITY;
       }
-      // running maximum and sum; the weights carry a factor of 4 (p <= 4), which
-      // l carries too: p d stays an fp16 value for every d below 2^14
+      // Running maximum and sum.  The maximum follows only when a score leads it
+      // by more than 2^8: the weights are 2^(s - max - 6), so at most 4, and p d stays
+      // an fp16 value for every d below 2^14; the factor is l's too.
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float top = mx[nt];
+        float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, sT[nt][i >> 2][(i >> 1) & 1][i & 1]);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if (__any_sync(0xffffffffu, top != mx[nt])) {
+        if (__any_sync(0xffffffffu, top > mx[nt] + slack[nt])) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          top = fmaxf(top, mx[nt]);
           const float f = top == mx[nt] ? 1.f : ex2((mx[nt] - top) * cs[nt]);
           l[nt] *= f;
           const float f0 = __shfl_sync(0xffffffffu, f, 8 * t4),
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
           }
           mx[nt] = top;
         }
-        const float base = fmaf(top == -INFINITY ? 0.f : top, -cs[nt], 2.f);
+        const float base = fmaf(mx[nt] == -INFINITY ? 0.f : mx[nt], -cs[nt], -6.f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float &v = sT[nt][i >> 2][(i >> 1) & 1][i & 1];
@@ -543,24 +543,29 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
         }
       }
     };
-    if (masked)
-      block(std::true_type());
-    else
-      block(std::false_type());
-    __syncwarp();  // every lane is done with the stage
-    if (issued < w1) {
-      issue(ahead, stage);
-      ++issued;
+    for (; cur.blk < end_blk; ++cur.blk) {
+      // after a wait that ran out (status is set) the rest is only walked through
+      if (ok) ok = mbar_wait_bounded(bar0 + 8 * stage, phase, a.status);
+      if (cur.blk >= mask_from)
+        block(std::true_type());
+      else
+        block(std::false_type());
+      __syncwarp();  // every lane is done with the stage
+      if (to_copy > 0) copy(stage);
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
 
-    // the item or the stretch ends: its output, or a piece of it
-    const bool item_ends = cur.blk + 1 == cur.nb;
-    if (item_ends || x + 1 == w1) {
+    // the item or the stretch ends: the item's output, or a piece of it
+    {
+      const bool item_ends = cur.blk == cur.nb;
       const int item = x - cur.blk;  // the item's first block on the line
-      const bool whole = item_ends && first == item;
-      const int slot = 2 * warp + (x + 1 == w1 ? 1 : 0);
-      float *piece = x + 1 == w1 ? reinterpret_cast<float *>(smem + warp * STAGES * kStage)
-                                 : s_head + warp * kPiece;
+      const bool whole = item_ends && first_blk == 0;
+      const int slot = 2 * warp + (x == w1 ? 1 : 0);
+      float *piece = x == w1 ? reinterpret_cast<float *>(smem + warp * STAGES * kStage)
+                             : s_head + warp * kPiece;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int count = cur.count;
@@ -623,12 +628,13 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
         s_item[slot] = item;
         s_bh[slot] = cur.b * a.n_kv + cur.h;
       }
+      if (item_ends && x < w1) next_item(cur);
     }
-    next(cur);
   }
-  if (!ok)  // status is set; let this warp's copies land before its shared memory goes
-    for (int s = 0; s < STAGES && s < issued - w0; ++s)
-      mbar_wait_bounded(bar0 + 8 * s, (uint32_t)((issued - w0 - 1 - s) / STAGES) & 1, a.status);
+  if (!ok) {  // let this warp's last copies land before its shared memory goes
+    for (int i = 0; i < min(STAGES, w1 - w0); ++i)
+      mbar_wait_bounded(bar0 + 8 * i, (uint32_t)((w1 - w0 - 1 - i) / STAGES) & 1, a.status);
+  }
   __syncthreads();
 
   // Join the pieces.  A slot per lane; an item's pieces are one per warp of a
@@ -699,18 +705,26 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
         auto part_of = [&](int c) {
           return a.parts + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kMaxCols * kPieceRow + col * kPieceRow;
         };
-        float top = -INFINITY;
-        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(part_of(c) + kD));
-        top = warp_max(top);
-        float v = 0.f, sum = 0.f;
+        float top = -INFINITY, v = 0.f, sum = 0.f;
+        // 32 parts at a time, their statistics one per lane; a new maximum rescales
         for (int cb = c0; cb <= c1; cb += 32) {
-          const int c = min(cb + lane, c1), k1 = min(32, c1 - cb + 1);
-          const float m = __ldcg(part_of(c) + kD);
-          const float f = cb + lane > c1 ? 0.f : m == top ? 1.f : ex2(m - top);
-          sum += cb + lane > c1 ? 0.f : f * __ldcg(part_of(c) + kD + 1);
-#pragma unroll 8
-          for (int k = 0; k < k1; ++k)
-            v = fmaf(__shfl_sync(0xffffffffu, f, k), __ldcg(part_of(cb + k) + d), v);
+          const int n1 = min(32, c1 - cb + 1);
+          const bool in = lane < n1;
+          const float *ps = part_of(cb + (in ? lane : 0)) + kD;
+          const float m = in ? __ldcg(ps) : -INFINITY, ls = in ? __ldcg(ps + 1) : 0.f;
+          float w[8];
+          const float up = fmaxf(top, warp_max(m));
+          const float old = top == up ? 1.f : ex2(top - up), f = m == up ? 1.f : ex2(m - up);
+          v *= old;
+          sum = sum * old + (in ? f * ls : 0.f);
+          top = up;
+          for (int k0 = 0; k0 < n1; k0 += 8) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = k0 + k < n1 ? __ldcg(part_of(cb + k0 + k) + d) : 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (k0 + k < n1) v = fmaf(__shfl_sync(0xffffffffu, f, k0 + k), w[k], v);
+          }
         }
         sum = warp_sum(sum);
         emit(col, d, sum == 0.f ? 0.f : v / sum);
