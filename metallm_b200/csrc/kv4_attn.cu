@@ -4,22 +4,18 @@
 // and V the values m + d c the cache rows stand for (the fp16 cache's
 // counterpart is mlm_attn_decode; LlamaRunner.swift:669-952).
 //
-// Pointers to data that earlier kernels write carry no __restrict__, so that no
-// load of it moves above the dependent wait.
+// Up to 16 (token, head) rows per KV head here; more in kv4_attn_many.cu.
 #include <algorithm>
 #include <type_traits>
 
-#include "mlm_device.cuh"
-#include "mlm_internal.h"
+#include "kv4_common.cuh"
 #include "q4k_gemv_common.cuh"
 
 namespace mlm {
 namespace {
 
-constexpr int kRow = MLM_KV4_ROW_BYTES;
-constexpr int kD = 128;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kInvSqrtD = 0.08838834764831845f;
+constexpr int kRow = kKv4Row;
+constexpr int kD = kKv4D;
 
 // ---------------------------------------------------------------------------
 // Few rows: up to 16 (token, head) pairs of one KV head at once -- a decode
@@ -66,40 +62,6 @@ __device__ __forceinline__ void mma_f16_zero(float (&c)[4], uint32_t a0, uint32_
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-struct FewArgs {
-  const uint8_t *kc, *vc;
-  const __half *q;
-  void *out;
-  const int32_t *lens, *counts;
-  float *parts;   // [ctas][2][kMaxCols][kPieceRow]
-  int *arrivals;  // [ctas], zero between launches
-  int *status;
-  int batch, tokens, n_heads, n_kv, group, capacity;
-};
-
-// the sequence's rows and tokens, kept within the cache and the call
-__device__ __forceinline__ void seq_shape(const int32_t *lens, const int32_t *counts, int b,
-                                          int tokens, int capacity, int &len, int &count) {
-  len = min(max(lens[b], 0), capacity);
-  count = counts ? min(max(counts[b], 0), tokens) : tokens;
-}
-__device__ __forceinline__ bool seq_outside(const int32_t *lens, const int32_t *counts, int b,
-                                            int tokens, int capacity) {
-  return lens[b] < 0 || lens[b] > capacity || (counts && (counts[b] < 0 || counts[b] > tokens));
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t v) {
-  return __half22float2(*reinterpret_cast<const __half2 *>(&v));
-}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -131,9 +93,6 @@ __device__ __forceinline__ uint32_t lds4(uint32_t addr) {
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ float low_f16(uint32_t v) {
-  return __half2float(__ushort_as_half((unsigned short)v));
-}
 // the transpose of an 8x8 matrix of 16-bit elements, row r of it in lanes 4r ..
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
@@ -148,10 +107,6 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_
       "l"(src), "r"(bytes), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ uint32_t u4_get(const uint4 &v, int i) {
-  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
-}
-
 // an item (the blocks of one KV head of one sequence) and a block of it
 struct Item {
   int b, h, blk, nb;
@@ -159,7 +114,7 @@ struct Item {
 };
 
 template <int NT, bool DUP, int W, int STAGES, class OutT>
-__global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
+__global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) {
   static_assert(2 * W <= 32, "a lane per piece");
   static_assert(!DUP || NT == 1, "hi and lo share one tile of columns");
   constexpr int kCols = DUP ? 4 : 8 * NT;
@@ -196,9 +151,9 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
       int n = 0;
       if (b < a.batch) {
         int len, count;
-        seq_shape(a.lens, a.counts, b, a.tokens, a.capacity, len, count);
+        seq_shape(a, b, len, count);
         n = count > 0 ? (len + kBlk - 1) / kBlk * a.n_kv : 0;
-        if (blockIdx.x == 0 && seq_outside(a.lens, a.counts, b, a.tokens, a.capacity))
+        if (blockIdx.x == 0 && seq_outside(a, b))
           *a.status = MLM_ERR_SHAPE;
       }
       int in = n;
@@ -218,7 +173,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
     if (s_off[b + 1] > s_off[b]) continue;
     int len, count;
-    seq_shape(a.lens, a.counts, b, a.tokens, a.capacity, len, count);
+    seq_shape(a, b, len, count);
     OutT *o = reinterpret_cast<OutT *>(a.out) + (size_t)b * a.tokens * a.n_heads * kD;
     for (int i = threadIdx.x; i < count * a.n_heads * kD; i += W * 32) o[i] = from_float<OutT>(0.f);
   }
@@ -238,7 +193,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
     }
     Item c;
     c.b = lo;
-    seq_shape(a.lens, a.counts, lo, a.tokens, a.capacity, c.len, c.count);
+    seq_shape(a, lo, c.len, c.count);
     c.nb = (c.len + kBlk - 1) / kBlk;
     const int rem = x - s_off[lo];
     c.h = rem / c.nb;
@@ -251,7 +206,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
     c.h = 0;
     do ++c.b; while (c.b < a.batch && s_off[c.b + 1] == s_off[c.b]);
     if (c.b == a.batch) return;
-    seq_shape(a.lens, a.counts, c.b, a.tokens, a.capacity, c.len, c.count);
+    seq_shape(a, c.b, c.len, c.count);
     c.nb = (c.len + kBlk - 1) / kBlk;
   };
   auto source = [&](const Item &c) {
@@ -653,7 +608,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(FewArgs a) {
     const int nb = (s_off[b + 1] - s_off[b]) / a.n_kv;
     const bool complete = item >= cta0 && item + nb <= cta1;
     int len, count;
-    seq_shape(a.lens, a.counts, b, a.tokens, a.capacity, len, count);
+    seq_shape(a, b, len, count);
     auto piece_of = [&](int i) -> const float * {  // of warp first_warp + i
       return i == n - 1 && !(s1 & 1)
                  ? s_head + (first_warp + i) * kPiece
@@ -754,7 +709,7 @@ constexpr auto few_kernel() {
 }
 
 template <int NT, bool DUP, class OutT>
-int few_launch(mlm_ctx *ctx, const FewArgs &a) {
+int few_launch(mlm_ctx *ctx, const Kv4AttnArgs &a) {
   using S = FewShape<NT, DUP>;
   return check_launch_pdl(ctx,
                           launch_pdl(few_kernel<NT, DUP, OutT>(), dim3(ctx->sm_count),
@@ -762,74 +717,11 @@ int few_launch(mlm_ctx *ctx, const FewArgs &a) {
                           "mlm_attn_kv4");
 }
 template <class OutT>
-int few(mlm_ctx *ctx, const FewArgs &a) {
+int few(mlm_ctx *ctx, const Kv4AttnArgs &a) {
   const int cols = a.tokens * a.group;
   if (cols <= 4) return few_launch<1, true, OutT>(ctx, a);
   if (cols <= 8) return few_launch<1, false, OutT>(ctx, a);
   return few_launch<2, false, OutT>(ctx, a);
-}
-
-// the lane's four values of a cache row
-__device__ __forceinline__ float4 row4(const uint8_t *row, int lane) {
-  const uint32_t w = *reinterpret_cast<const uint16_t *>(row + 2 * lane);
-  const float2 dm = __half22float2(*reinterpret_cast<const __half2 *>(row + 64 + 4 * (lane / 8)));
-  return make_float4(fmaf(dm.x, (float)(w & 15u), dm.y), fmaf(dm.x, (float)((w >> 4) & 15u), dm.y),
-                     fmaf(dm.x, (float)((w >> 8) & 15u), dm.y), fmaf(dm.x, (float)(w >> 12), dm.y));
-}
-
-// Many rows: one warp per (sequence, token, query head) walks the rows the token
-// sees with a running maximum and sum; a lane holds dimensions 4l .. 4l+3.
-template <class OutT>
-__global__ void __launch_bounds__(128) kv4_attn_simple_kernel(
-    const uint8_t *kc, const uint8_t *vc, const __half *q, OutT *out, int batch, int tokens,
-    int n_heads, int n_kv, int capacity, const int32_t *lens, const int32_t *counts, int *status) {
-  pdl_wait_then_release();
-  const long long i = (long long)blockIdx.x * 4 + threadIdx.x / 32;
-  const int lane = threadIdx.x & 31;
-  if (i >= (long long)batch * tokens * n_heads) return;
-  const int head = (int)(i % n_heads);
-  const int t = (int)(i / n_heads % tokens);
-  const int b = (int)(i / n_heads / tokens);
-  int len, count;
-  seq_shape(lens, counts, b, tokens, capacity, len, count);
-  if (lane == 0 && seq_outside(lens, counts, b, tokens, capacity)) *status = MLM_ERR_SHAPE;
-  if (t >= count) return;
-  const int seen = max(0, len - count + t + 1);
-  const size_t at = (size_t)i * kD + 4 * lane;
-  float x[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = __half2float(q[at + e]);
-  const size_t row0 = ((size_t)b * n_kv + head / (n_heads / n_kv)) * capacity;
-  float top = -INFINITY, sum = 0.f, o[4] = {};
-  for (int j = 0; j < seen; ++j) {
-    const float4 k = row4(kc + (row0 + j) * kRow, lane);
-    const float s = warp_sum(x[0] * k.x + x[1] * k.y + x[2] * k.z + x[3] * k.w) * kInvSqrtD;
-    const float up = fmaxf(top, s);
-    const float old = top == up ? 1.f : expf(top - up), p = expf(s - up);
-    const float4 v = row4(vc + (row0 + j) * kRow, lane);
-    o[0] = o[0] * old + p * v.x;
-    o[1] = o[1] * old + p * v.y;
-    o[2] = o[2] * old + p * v.z;
-    o[3] = o[3] * old + p * v.w;
-    sum = sum * old + p;
-    top = up;
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) out[at + e] = from_float<OutT>(seen ? o[e] / sum : 0.f);
-}
-
-template <class OutT>
-int simple(mlm_ctx *ctx, const mlm_kv4_cache &c, const void *q, int n_heads, int tokens,
-           const int32_t *lens, const int32_t *counts, void *out) {
-  const long long warps = (long long)c.batch * tokens * n_heads;
-  return check_launch_pdl(
-      ctx,
-      launch_pdl(kv4_attn_simple_kernel<OutT>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0,
-                 ctx->stream, reinterpret_cast<const uint8_t *>(c.k),
-                 reinterpret_cast<const uint8_t *>(c.v), reinterpret_cast<const __half *>(q),
-                 reinterpret_cast<OutT *>(out), c.batch, tokens, n_heads, c.n_kv_heads, c.capacity,
-                 lens, counts, ctx->dev_status),
-      "mlm_attn_kv4");
 }
 
 template <int NT, bool DUP, class OutT>
@@ -849,13 +741,19 @@ int kv4_attn_init(mlm_ctx *ctx) {
   if (st == MLM_OK) st = few_init<1, true, __nv_bfloat16>(ctx);
   if (st == MLM_OK) st = few_init<1, false, __nv_bfloat16>(ctx);
   if (st == MLM_OK) st = few_init<2, false, __nv_bfloat16>(ctx);
+  if (st == MLM_OK) st = kv4_attn_many_init(ctx);
   if (st != MLM_OK) return st;
-  const size_t parts = sizeof(float) * 2 * ctx->sm_count * kMaxCols * kPieceRow;
+  const size_t parts = std::max(sizeof(float) * 2 * ctx->sm_count * kMaxCols * kPieceRow,
+                                kv4_many_parts_bytes(ctx->sm_count));
   if (cudaMalloc(&ctx->kv4_parts, parts) != cudaSuccess ||
-      cudaMalloc(&ctx->kv4_arrivals, sizeof(int) * ctx->sm_count) != cudaSuccess)
+      cudaMalloc(&ctx->kv4_arrivals, sizeof(int) * (ctx->sm_count + 1 + kKv4PlanInts)) != cudaSuccess)
     return set_error(ctx, MLM_ERR_ALLOC, "mlm_attn_kv4: scratch");
   MLM_CUDA_TRY(ctx, cudaMemset(ctx->kv4_arrivals, 0, sizeof(int) * ctx->sm_count));
   return MLM_OK;
+}
+
+int kv4_attn_few(mlm_ctx *ctx, const Kv4AttnArgs &a, int out_type) {
+  return out_type == MLM_TYPE_F16 ? few<__half>(ctx, a) : few<__nv_bfloat16>(ctx, a);
 }
 
 }  // namespace mlm
@@ -882,26 +780,23 @@ extern "C" int mlm_attn_kv4(mlm_ctx *ctx, const mlm_kv4_cache *cache, const void
               "mlm_attn_kv4: tokens=%d (1 .. 65536)", tokens);
   DeviceGuard guard(ctx);
   const int group = n_heads / cache->n_kv_heads;
-  if ((long long)tokens * group <= kMaxCols) {
-    FewArgs a;
-    a.kc = reinterpret_cast<const uint8_t *>(cache->k);
-    a.vc = reinterpret_cast<const uint8_t *>(cache->v);
-    a.q = reinterpret_cast<const __half *>(q);
-    a.out = out;
-    a.lens = lens;
-    a.counts = counts;
-    a.parts = ctx->kv4_parts;
-    a.arrivals = ctx->kv4_arrivals;
-    a.status = ctx->dev_status;
-    a.batch = cache->batch;
-    a.tokens = tokens;
-    a.n_heads = n_heads;
-    a.n_kv = cache->n_kv_heads;
-    a.group = group;
-    a.capacity = cache->capacity;
-    return out_type == MLM_TYPE_F16 ? few<__half>(ctx, a) : few<__nv_bfloat16>(ctx, a);
-  }
-  if (out_type == MLM_TYPE_F16)
-    return simple<__half>(ctx, *cache, q, n_heads, tokens, lens, counts, out);
-  return simple<__nv_bfloat16>(ctx, *cache, q, n_heads, tokens, lens, counts, out);
+  Kv4AttnArgs a;
+  a.kc = reinterpret_cast<const uint8_t *>(cache->k);
+  a.vc = reinterpret_cast<const uint8_t *>(cache->v);
+  a.q = reinterpret_cast<const __half *>(q);
+  a.out = out;
+  a.lens = lens;
+  a.counts = counts;
+  a.parts = ctx->kv4_parts;
+  a.arrivals = ctx->kv4_arrivals;
+  a.plan = ctx->kv4_arrivals + (ctx->sm_count + 1) / 2 * 2;
+  a.status = ctx->dev_status;
+  a.batch = cache->batch;
+  a.tokens = tokens;
+  a.n_heads = n_heads;
+  a.n_kv = cache->n_kv_heads;
+  a.group = group;
+  a.capacity = cache->capacity;
+  return (long long)tokens * group <= kMaxCols ? kv4_attn_few(ctx, a, out_type)
+                                               : kv4_attn_many(ctx, a, out_type);
 }

@@ -1,0 +1,675 @@
+// kv4_attn_many.cu -- attention over the 4-bit KV cache for many rows: prompt
+// chunks, and more than 16 (token, head) pairs per KV head in general.
+//
+// The rows of one (sequence, KV head) are its (token, query head of the group)
+// pairs, token first, so a group's heads share every key tile.  A CTA takes 256
+// rows (two tiles of 128) against tiles of 128 keys, both products on tcgen05
+// with fp32 accumulators in TMEM (M = N = 128):
+//   - 4 warps turn a key tile's cache rows into fp16 K and V in shared memory
+//     (a thread per key; one rounding of m + d c, as the read-back gives it), two
+//     buffers;
+//   - one thread issues S = Q K^T and O += P V, the two row tiles in turn, so
+//     that one tile's softmax runs while the other's products do;
+//   - 4 warps per row tile do the softmax, a thread per row: S from TMEM, the
+//     weights back as fp16 over it, where the second product reads them as its A
+//     operand.
+// The running maximum follows only when a score leads it by more than 2^8 (a
+// weight is then at most 2^8, an fp16 value), so the accumulator in TMEM is
+// rescaled once in a row's life, as a rule.  Scores, maxima and sums are fp32;
+// K, V and the weights are fp16 operands.
+//
+// V^T is the N-major B operand of the second product: both K and V lie in
+// shared memory as [key][dimension] in the 128-byte swizzle, the eight
+// elements of a code word in the order its masks give (0 4 1 5 2 6 3 7); Q is
+// stored in the same order and the output columns are put back.
+//
+// The tiles of all (sequence, 256 rows, KV head) items form one line that is cut
+// into equal stretches, one per CTA, from the lengths in device memory.  An item
+// that several CTAs share leaves fp32 parts in the context's scratch, which a
+// second kernel joins in order.
+//
+// A NaN in a cache row reaches every token that sees the row and no other: a
+// masked weight is 0, but 0 x NaN is not, so a value row with NaN scales goes in
+// as zeros and makes its key NaN instead.
+#include <algorithm>
+#include <type_traits>
+
+#include "kv4_common.cuh"
+#include "q4k_gemv_common.cuh"
+
+namespace mlm {
+namespace {
+
+constexpr int kTile = 128;          // rows of a row tile, keys of a key tile
+constexpr int kRows = 2 * kTile;    // rows of an item
+constexpr int kSoftWarps = 8, kDqWarps = 4;
+constexpr int kThreads = 32 * (kSoftWarps + kDqWarps + 1);
+constexpr int kSub = kTile * 128;           // 64 dimensions of a tile: 128 rows x 128 bytes
+constexpr int kOperand = 2 * kSub;          // 32 KB: Q, K or V of a tile
+constexpr int kOffKv = 2 * kOperand;        // after Q of two tiles
+constexpr int kOffBar = kOffKv + 4 * kOperand;
+enum { kQfull = 0, kSfull = 1, kPfull = 3, kOfull = 5, kKvFull = 7, kKvEmpty = 9, kDrain = 11, kBars = 12 };
+constexpr int kOffTmem = kOffBar + 8 * kBars;
+constexpr int kOffLine = kOffTmem + 16;     // [batch + 1] 64-bit offsets
+constexpr size_t smem_bytes(int batch) { return kOffLine + 8 * (size_t)(batch + 1); }
+constexpr int kTmemCols = 512;  // S/P of tile 0 and 1, O of tile 0 and 1
+constexpr int kPartRow = kKv4D + 4;  // a row of a part: o[128], m, l, padding
+constexpr float kScale2 = kInvSqrtD * kLog2e;
+constexpr float kLead = 8.f / kScale2;
+
+// instruction descriptors: fp16 A and B, fp32 accumulators, M = N = 128; B K-major
+// (S = Q K^T) or N-major (O = P V)
+constexpr uint32_t kIdescS = (1u << 4) | ((kTile >> 3) << 17) | ((kTile >> 4) << 24);
+constexpr uint32_t kIdescO = kIdescS | (1u << 16);
+
+// Matrix descriptors of the 128-byte swizzle: rows of 128 bytes in 8-row atoms
+// of 1024 bytes, 16-byte chunk c of row r at c ^ (r & 7); version 1, layout type
+// 2.  K-major: atoms 1024 bytes apart along the rows.  N-major: 8-key groups
+// 1024 bytes apart, 64-dimension halves kSub bytes apart.
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_n_major(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kSub >> 4) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// byte offset of 16-byte chunk c (0 .. 15) of row r in an operand
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  return (uint32_t)((c >> 3) * kSub + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(kIdescS), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(kIdescO), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                   bar)
+               : "memory");
+}
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+        "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+      "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]),
+      "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
+      "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+// packed fp32 pairs
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ int row_tiles(int count, int group) {
+  return (count * group + kRows - 1) / kRows;
+}
+// key tiles of a sequence's rt-th 256 rows: up to what their last token sees
+__device__ __forceinline__ int key_tiles(int len, int count, int group, int rt) {
+  const int last = min(count - 1, ((rt + 1) * kRows - 1) / group);
+  return max(0, (len - count + last + 1 + kTile - 1) / kTile);
+}
+
+// Key tiles kt0 .. kt1 of nkt of an item: a CTA's stretch is a sequence of these,
+// which every role walks alike.
+struct Part {
+  int b, rt, h, kt0, kt1, nkt, len, count;
+};
+struct Walk {
+  const Kv4AttnArgs &a;
+  const long long *off;  // the line's offsets per sequence
+  long long x, x1;
+  Part p;
+  __device__ Walk(const Kv4AttnArgs &a_, const long long *off_, long long x0, long long x1_)
+      : a(a_), off(off_), x(x0), x1(x1_), p{} {
+    if (x >= x1) return;
+    int lo = 0, hi = a.batch;  // the last sequence with off <= x
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (off[mid] <= x) lo = mid; else hi = mid;
+    }
+    p.b = lo;
+    seq_shape(a, lo, p.len, p.count);
+    long long y = x - off[lo];
+    for (;; ++p.rt) {
+      p.nkt = key_tiles(p.len, p.count, a.group, p.rt);
+      const long long span = (long long)p.nkt * a.n_kv;
+      if (y < span) break;
+      y -= span;
+    }
+    p.h = (int)(y / p.nkt);
+    p.kt1 = (int)(y - (long long)p.h * p.nkt);  // where the first part begins
+    --p.h;  // next() moves on from the item before
+    first = true;
+  }
+  bool first = false;
+  __device__ bool next() {
+    if (x >= x1) return false;
+    const int begin = first ? p.kt1 : 0;
+    first = false;
+    if (++p.h == a.n_kv) {
+      p.h = 0;
+      do {
+        ++p.rt;
+        while (p.rt >= row_tiles(p.count, a.group) || off[p.b + 1] == off[p.b]) {
+          ++p.b;
+          p.rt = 0;
+          seq_shape(a, p.b, p.len, p.count);
+        }
+        p.nkt = key_tiles(p.len, p.count, a.group, p.rt);
+      } while (p.nkt == 0);
+    }
+    p.kt0 = begin;
+    p.kt1 = (int)min((long long)p.nkt, begin + (x1 - x));
+    x += p.kt1 - p.kt0;
+    return true;
+  }
+};
+
+// one word of codes to eight fp16 values in the order 0 4 1 5 2 6 3 7
+__device__ __forceinline__ uint4 values8(uint32_t w, __half2 d, __half2 m) {
+  // codes in the mantissa of 1024 (of 64 where they sit 4 bits higher)
+  const __half2 one = __float2half2_rn(-1024.f), low = __float2half2_rn(-64.f),
+                sixteenth = __float2half2_rn(0.0625f);
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = i ? w >> 8 : w;
+    const uint32_t a = (x & 0x000F000Fu) | 0x64006400u, b = (x & 0x00F000F0u) | 0x64006400u;
+    const __half2 ca = __hadd2(*reinterpret_cast<const __half2 *>(&a), one);
+    const __half2 cb = __hfma2(*reinterpret_cast<const __half2 *>(&b), sixteenth, low);
+    const __half2 va = __hfma2(ca, d, m), vb = __hfma2(cb, d, m);
+    v[2 * i] = *reinterpret_cast<const uint32_t *>(&va);
+    v[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&vb);
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ bool not_finite(uint32_t dm) {
+  return (dm & 0x7C00u) == 0x7C00u || (dm & 0x7C000000u) == 0x7C000000u;
+}
+
+template <class OutT>
+__global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sbase = (uint32_t)__cvta_generic_to_shared(smem);
+  const uint32_t bar = sbase + kOffBar;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + kOffTmem);
+  long long *s_off = reinterpret_cast<long long *>(smem + kOffLine);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(bar + 8 * kQfull, 32 * kSoftWarps);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar + 8 * (kSfull + i), 1);
+      mbar_init(bar + 8 * (kPfull + i), kTile);
+      mbar_init(bar + 8 * (kOfull + i), 1);
+      mbar_init(bar + 8 * (kKvFull + i), kDqWarps);
+      mbar_init(bar + 8 * (kKvEmpty + i), 1);
+    }
+    mbar_init(bar + 8 * kDrain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kSoftWarps + kDqWarps) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     (uint32_t)__cvta_generic_to_shared(tmem_slot)),
+                 "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pdl_wait_then_release();
+
+  // the line: key tiles per sequence, then their running sum
+  for (int b = warp; b < a.batch; b += kThreads / 32) {
+    int len, count;
+    seq_shape(a, b, len, count);
+    long long n = 0;
+    for (int rt = lane; rt < row_tiles(count, a.group); rt += 32)
+      n += (long long)key_tiles(len, count, a.group, rt) * a.n_kv;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    if (lane == 0) {
+      s_off[b + 1] = n;
+      if (blockIdx.x == 0 && seq_outside(a, b)) *a.status = MLM_ERR_SHAPE;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (threadIdx.x == 0) {
+    long long run = 0;
+    s_off[0] = 0;
+    for (int b = 1; b <= a.batch; ++b) s_off[b] = run += s_off[b];
+  }
+  __syncthreads();
+  const uint32_t tmem = *tmem_slot;
+  const long long total = s_off[a.batch];
+  const long long quota = max(4ll, (total + gridDim.x - 1) / gridDim.x);
+  const long long x0 = min(total, blockIdx.x * quota), x1 = min(total, x0 + quota);
+  if (blockIdx.x == 0) {  // the cut, for the joining kernel
+    long long *plan = reinterpret_cast<long long *>(a.plan);
+    if (threadIdx.x == 0) plan[0] = quota;
+    for (int b = threadIdx.x; b <= a.batch; b += kThreads) plan[1 + b] = s_off[b];
+  }
+  // tokens that attend to nothing: the first count - len of a sequence
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    int len, count;
+    seq_shape(a, b, len, count);
+    OutT *o = reinterpret_cast<OutT *>(a.out) + (size_t)b * a.tokens * a.n_heads * kKv4D;
+    const long long n = (long long)max(0, count - len) * a.n_heads * kKv4D;
+    for (long long i = threadIdx.x; i < n; i += kThreads) o[i] = from_float<OutT>(0.f);
+  }
+
+  Walk walk(a, s_off, x0, x1);
+  bool ok = true;
+  if (warp < kSoftWarps) {
+    // ---- softmax: a thread per row of tile `tile` --------------------------------
+    const int tile = warp >> 2, r = threadIdx.x & (kTile - 1);
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + tile * kTile, to = tmem + lanes + (2 + tile) * kTile;
+    uint32_t n_s = 0, n_q = 0, n_item = 0;
+    while (ok && walk.next()) {
+      const Part p = walk.p;
+      const int live = p.count * a.group - p.rt * kRows;  // rows of the item
+      const int row = p.rt * kRows + tile * kTile + r;
+      const bool mine = tile * kTile + r < live;
+      const int tok = mine ? row / a.group : 0;
+      const int seen = mine ? max(0, p.len - p.count + tok + 1) : 0;
+      const size_t at = (((size_t)p.b * a.tokens + tok) * a.n_heads + p.h * a.group +
+                         (row - tok * a.group)) * kKv4D;
+      // the row's q, in the order of the codes
+      {
+        const uint4 *src = reinterpret_cast<const uint4 *>(a.q + at);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const uint4 v = mine ? src[c] : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4 *>(smem + tile * kOperand + chunk_at(r, c)) =
+              make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                         __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc_fence_before();
+        arrive(bar + 8 * kQfull);
+      }
+      if (tile * kTile >= live) {  // no row of this tile: its products do not run
+        // not past the other tile: its arrivals for this item come first
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar + 8 * kQfull, n_q++ & 1, a.status));
+        continue;
+      }
+      ++n_q;
+      float m = -INFINITY;
+      uint64_t l2 = 0;
+      for (int kt = p.kt0; kt < p.kt1; ++kt) {
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait_bounded(bar + 8 * (kSfull + tile), n_s & 1, a.status));
+        if (!ok) break;
+        ++n_s;
+        tc_fence_after();
+        const int lim = seen - kt * kTile;  // keys of the tile that the row sees
+        uint32_t w[64];
+        uint64_t sum = 0;
+        // weights against the maximum m; returns the tile's largest score
+        auto weights = [&](auto mask_tag) {
+          constexpr bool MASK = decltype(mask_tag)::value;
+          const float m2 = m == -INFINITY ? 0.f : -m * kScale2;
+          const uint64_t mm = pair(m2, m2), cc = pair(kScale2, kScale2);
+          float top0 = -INFINITY, top1 = -INFINITY;
+          sum = 0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t s[32];
+            tmem_ld32(ts + 32 * c, s);
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+              float s0 = __uint_as_float(s[k]), s1 = __uint_as_float(s[k + 1]);
+              if (MASK) {
+                if (32 * c + k >= lim) s0 = -INFINITY;
+                if (32 * c + k + 1 >= lim) s1 = -INFINITY;
+              }
+              top0 = fmaxf(top0, s0);
+              top1 = fmaxf(top1, s1);
+              const float2 e = unpair(fma2(pair(s0, s1), cc, mm));
+              const float p0 = ex2(e.x), p1 = ex2(e.y);
+              sum = add2(sum, pair(p0, p1));
+              w[16 * c + k / 2] = pack_f16(p0, p1);
+            }
+          }
+          return fmaxf(top0, top1);
+        };
+        const bool masked = __any_sync(0xffffffffu, lim < kTile);
+        const float top = masked ? weights(std::true_type()) : weights(std::false_type());
+        if (__any_sync(0xffffffffu, top > m + kLead)) {
+          const float up = fmaxf(m, top);
+          const float f = up == m ? 1.f : ex2((m - up) * kScale2);
+          if (kt > p.kt0) {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[32];
+              tmem_ld32(to + 32 * c, o);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st32(to + 32 * c, o);
+            }
+          }
+          const float2 l = unpair(l2);
+          l2 = pair(l.x * f, l.y * f);
+          m = up;
+          if (masked)
+            weights(std::true_type());
+          else
+            weights(std::false_type());
+        }
+        l2 = add2(l2, sum);
+        tmem_st32(ts, w);
+        tmem_st32(ts + 32, w + 32);
+        tmem_wait_st();
+        tc_fence_before();
+        arrive(bar + 8 * (kPfull + tile));
+      }
+      if (!ok) break;
+      ok = __all_sync(0xffffffffu,
+                      mbar_wait_bounded(bar + 8 * (kOfull + tile), n_item & 1, a.status));
+      if (!ok) break;
+      ++n_item;
+      tc_fence_after();
+      const float2 l = unpair(l2);
+      const float sum = l.x + l.y;
+      const long long item = walk.x - p.kt1;  // the item's first tile on the line
+      const bool whole = p.kt0 == 0 && p.kt1 == p.nkt;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      float *part = a.parts + (((size_t)blockIdx.x * 2 + (item < x0 ? 0 : 1)) * kRows +
+                               tile * kTile + r) * kPartRow;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        tmem_ld32(to + 32 * c, o);
+        if (mine) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float e[8];  // columns 0 4 1 5 2 6 3 7 back in order
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[(k >> 1) + 4 * (k & 1)] = __uint_as_float(o[8 * j + k]);
+            if (whole) {
+              OutT h[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) h[k] = from_float<OutT>(e[k] * inv);
+              *reinterpret_cast<uint4 *>(reinterpret_cast<OutT *>(a.out) + at + 32 * c + 8 * j) =
+                  *reinterpret_cast<const uint4 *>(h);
+            } else {
+              float4 *dst = reinterpret_cast<float4 *>(part + 32 * c + 8 * j);
+              dst[0] = make_float4(e[0], e[1], e[2], e[3]);
+              dst[1] = make_float4(e[4], e[5], e[6], e[7]);
+            }
+          }
+        }
+        __syncwarp();
+      }
+      if (!whole && mine) {
+        part[kKv4D] = m * kScale2;
+        part[kKv4D + 1] = sum;
+      }
+    }
+  } else if (warp < kSoftWarps + kDqWarps) {
+    // ---- cache rows to fp16 operands: a thread per key of the tile ----------------
+    const int key = threadIdx.x - 32 * kSoftWarps;
+    uint32_t n_kv = 0;
+    uint4 raw[10];
+    auto load = [&](const Part &p, int kt) {
+      const int j = kt * kTile + key;
+      if (j < p.len) {
+        const size_t at = (((size_t)p.b * a.n_kv + p.h) * a.capacity + j) * kKv4Row;
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+          raw[i] = *reinterpret_cast<const uint4 *>(a.kc + at + 16 * i);
+          raw[5 + i] = *reinterpret_cast<const uint4 *>(a.vc + at + 16 * i);
+        }
+      } else {  // past the sequence: zeros
+#pragma unroll
+        for (int i = 0; i < 10; ++i) raw[i] = make_uint4(0, 0, 0, 0);
+      }
+    };
+    bool more = walk.next();
+    int kt = walk.p.kt0;
+    if (more) load(walk.p, kt);
+    while (more) {
+      const uint32_t buf = n_kv & 1;
+      if (n_kv >= 2) {
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar + 8 * (kKvEmpty + buf),
+                                                       ((n_kv >> 1) - 1) & 1, a.status));
+        if (!ok) break;
+      }
+      uint4 cur[10];
+#pragma unroll
+      for (int i = 0; i < 10; ++i) cur[i] = raw[i];
+      if (++kt == walk.p.kt1) {
+        more = walk.next();
+        kt = walk.p.kt0;
+      }
+      if (more) load(walk.p, kt);
+      const bool bad = not_finite(cur[9].x) || not_finite(cur[9].y) || not_finite(cur[9].z) ||
+                       not_finite(cur[9].w);
+      if (bad) {
+#pragma unroll
+        for (int i = 5; i < 10; ++i) cur[i] = make_uint4(0, 0, 0, 0);
+        cur[4] = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
+      }
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        uint8_t *dst = smem + kOffKv + (2 * buf + kv) * kOperand;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const uint32_t dm = u4_get(cur[5 * kv + 4], g);
+          const uint32_t dd = __byte_perm(dm, dm, 0x1010), mm = __byte_perm(dm, dm, 0x3232);
+          const __half2 d = *reinterpret_cast<const __half2 *>(&dd),
+                        m = *reinterpret_cast<const __half2 *>(&mm);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4 *>(dst + chunk_at(key, 4 * g + i)) =
+                values8(u4_get(cur[5 * kv + g], i), d, m);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive(bar + 8 * (kKvFull + buf));
+      ++n_kv;
+    }
+  } else if (lane == 0) {
+    // ---- the products -----------------------------------------------------------
+    uint32_t n_kv = 0, n_p[2] = {0, 0}, n_item = 0;
+    auto scores = [&](int tile, uint32_t buf) {
+      const uint32_t qa = sbase + tile * kOperand, ka = sbase + kOffKv + 2 * buf * kOperand;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t o = (k >> 2) * kSub + (k & 3) * 32;
+        mma_smem(tmem + tile * kTile, desc_k_major(qa + o), desc_k_major(ka + o), k > 0);
+      }
+      commit(bar + 8 * (kSfull + tile));
+    };
+    auto kv_ready = [&](uint32_t n) {
+      return mbar_wait_bounded(bar + 8 * (kKvFull + (n & 1)), (n >> 1) & 1, a.status);
+    };
+    while (ok && walk.next()) {
+      const Part p = walk.p;
+      const int tiles = p.count * a.group - p.rt * kRows > kTile ? 2 : 1;
+      ok = mbar_wait_bounded(bar + 8 * kQfull, n_item & 1, a.status) && kv_ready(n_kv);
+      if (!ok) break;
+      ++n_item;
+      tc_fence_after();
+      for (int i = 0; i < tiles; ++i) scores(i, n_kv & 1);
+      for (int kt = p.kt0; ok && kt < p.kt1; ++kt, ++n_kv) {
+        const uint32_t va = sbase + kOffKv + (2 * (n_kv & 1) + 1) * kOperand;
+        for (int i = 0; i < tiles; ++i) {
+          ok = mbar_wait_bounded(bar + 8 * (kPfull + i), n_p[i] & 1, a.status);
+          if (!ok) break;
+          ++n_p[i];
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_tmem(tmem + (2 + i) * kTile, tmem + i * kTile + 8 * k, desc_n_major(va + 2048 * k),
+                     kt > p.kt0 || k > 0);
+          if (i == tiles - 1) commit(bar + 8 * (kKvEmpty + (n_kv & 1)));
+          if (kt + 1 < p.kt1) {
+            if (i == 0) {
+              ok = kv_ready(n_kv + 1);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            scores(i, (n_kv + 1) & 1);
+          } else {
+            commit(bar + 8 * (kOfull + i));
+          }
+        }
+      }
+    }
+    // nothing of this CTA is in flight when its TMEM and shared memory go
+    commit(bar + 8 * kDrain);
+    mbar_wait_bounded(bar + 8 * kDrain, 0, a.status);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kSoftWarps + kDqWarps) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+// Joins the parts of items that several CTAs shared: a warp per output row, four
+// dimensions per lane, the parts in order.
+template <class OutT>
+__global__ void __launch_bounds__(256) kv4_attn_join_kernel(Kv4AttnArgs a) {
+  pdl_wait_then_release();
+  const int lane = threadIdx.x & 31;
+  const long long *plan = reinterpret_cast<const long long *>(a.plan);
+  const long long rows = (long long)a.batch * a.tokens * a.n_heads;
+  const long long quota = plan[0];
+  for (long long i = (long long)blockIdx.x * 8 + threadIdx.x / 32; i < rows; i += gridDim.x * 8ll) {
+    const int head = (int)(i % a.n_heads), t = (int)(i / a.n_heads % a.tokens);
+    const int b = (int)(i / a.n_heads / a.tokens);
+    int len, count;
+    seq_shape(a, b, len, count);
+    if (t >= count) continue;
+    const int h = head / a.group, row = t * a.group + head - h * a.group, rt = row / kRows;
+    const int nkt = key_tiles(len, count, a.group, rt);
+    if (nkt == 0) continue;
+    long long before = 0;
+    for (int k = lane; k < rt; k += 32) before += key_tiles(len, count, a.group, k);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    const long long x = plan[1 + b] + before * a.n_kv + (long long)h * nkt;
+    const int c0 = (int)(x / quota), c1 = (int)((x + nkt - 1) / quota);
+    if (c0 == c1) continue;
+    float top = -INFINITY, sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      const float *p = a.parts + (((size_t)c * 2 + (c == c0 ? 1 : 0)) * kRows + (row - rt * kRows)) * kPartRow;
+      const float4 o = *reinterpret_cast<const float4 *>(p + 4 * lane);
+      const float m = p[kKv4D], l = p[kKv4D + 1];
+      const float up = fmaxf(top, m);
+      const float fo = top == up ? 1.f : ex2(top - up), f = m == up ? 1.f : ex2(m - up);
+      v.x = v.x * fo + f * o.x;
+      v.y = v.y * fo + f * o.y;
+      v.z = v.z * fo + f * o.z;
+      v.w = v.w * fo + f * o.w;
+      sum = sum * fo + f * l;
+      top = up;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    OutT e[4] = {from_float<OutT>(v.x * inv), from_float<OutT>(v.y * inv),
+                 from_float<OutT>(v.z * inv), from_float<OutT>(v.w * inv)};
+    *reinterpret_cast<uint2 *>(reinterpret_cast<OutT *>(a.out) + (size_t)i * kKv4D + 4 * lane) =
+        *reinterpret_cast<const uint2 *>(e);
+  }
+}
+
+template <class OutT>
+int many(mlm_ctx *ctx, const Kv4AttnArgs &a) {
+  const int st = check_launch_pdl(ctx,
+                                  launch_pdl(kv4_attn_many_kernel<OutT>, dim3(ctx->sm_count),
+                                             dim3(kThreads), smem_bytes(a.batch), ctx->stream, a),
+                                  "mlm_attn_kv4");
+  if (st != MLM_OK) return st;
+  const long long rows = (long long)a.batch * a.tokens * a.n_heads;
+  return check_launch_pdl(
+      ctx,
+      launch_pdl(kv4_attn_join_kernel<OutT>,
+                 dim3((unsigned)std::min<long long>((rows + 7) / 8, 8ll * ctx->sm_count)), dim3(256),
+                 0, ctx->stream, a),
+      "mlm_attn_kv4 (join)");
+}
+
+}  // namespace
+
+size_t kv4_many_parts_bytes(int sm_count) {
+  return sizeof(float) * 2 * sm_count * kRows * kPartRow;
+}
+
+int kv4_attn_many_init(mlm_ctx *ctx) {
+  MLM_CUDA_TRY(ctx, cudaFuncSetAttribute(kv4_attn_many_kernel<__half>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)smem_bytes(MLM_KV4_MAX_BATCH)));
+  MLM_CUDA_TRY(ctx, cudaFuncSetAttribute(kv4_attn_many_kernel<__nv_bfloat16>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)smem_bytes(MLM_KV4_MAX_BATCH)));
+  return MLM_OK;
+}
+
+int kv4_attn_many(mlm_ctx *ctx, const Kv4AttnArgs &a, int out_type) {
+  return out_type == MLM_TYPE_F16 ? many<__half>(ctx, a) : many<__nv_bfloat16>(ctx, a);
+}
+
+}  // namespace mlm

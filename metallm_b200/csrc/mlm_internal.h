@@ -42,7 +42,7 @@ struct mlm_ctx {
   int *attn_arrivals = nullptr;  // per (sequence, KV head); zero between launches
 
   // attention over the 4-bit cache: the CTAs' partial sums, and one arrival
-  // counter per CTA, zero between launches
+  // counter per CTA, zero between launches, then the cut of a many-row call
   float *kv4_parts = nullptr;
   int *kv4_arrivals = nullptr;
 
