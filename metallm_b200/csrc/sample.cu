@@ -9,15 +9,17 @@
 //  - masses are integers, w scaled to as many bits as the row's length leaves
 //    free, so sums do not depend on their order and a row's token does not
 //    depend on the run;
-//  - a pass puts every kept token into one of 2048 bins of (max - x), sums
-//    counts and masses per bin, and a scan finds the bin in which the k-th
-//    token, or the top_p share of the mass, falls; that bin's tokens (tens, in
-//    real logits) go into a list, are ranked, and give the exact cut.  A bin
-//    with more tokens than the list holds (flat or constant rows) is first
-//    narrowed by 11-bit digits of the key, which always ends, as keys are
+//  - a pass puts every token into one of 2048 bins of (max - x), sums counts or
+//    masses per bin, and a scan finds the bin in which the k-th token, or the
+//    top_p share of the mass, falls.  Where the tokens down to that bin fit a list
+//    (tens, for usual settings) they are gathered and one CTA does the rest on the
+//    list: ranks by counting, masses, both cuts and the draw.  Otherwise the bin's
+//    tokens alone are gathered and give the exact cut, and the draw goes over the
+//    row again; a bin with more tokens than the list holds (flat or constant rows)
+//    is first narrowed by 11-bit digits of the key, which always ends, as keys are
 //    distinct;
 //  - the draw is by index: masses per warp's stretch of the row, a scan, and the
-//    one stretch that holds the point is walked again.
+//    one stretch that holds the point is walked again by the whole CTA.
 // One cluster of CTAs per row; a CTA keeps its slice of the row in shared memory
 // (read once) where it fits and reads it again from L2 where it does not.
 #include <cooperative_groups.h>
@@ -34,18 +36,23 @@ namespace {
 
 using u64 = unsigned long long;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kCand = 1024;      // tokens of the list that is ranked
-constexpr int kMaxCluster = 8;
+constexpr int kCand = 1024;       // tokens of the list
+constexpr int kMaxCluster = 16;   // of CTAs; above 8 needs the opt-in
+constexpr int kMinSlice = 4096;   // tokens per CTA that are worth a CTA
 constexpr u64 kAll = 1ull << 32;  // the smallest key of a logit that is not NaN
 
 struct Shared {
+  double exp2_64[64];                         // 2^(j/64)
   uint32_t cnt[kBins], lo[kBins], hi[kBins];  // this CTA's bins; masses as 64 bits in halves
   uint32_t g_cnt[kBins];                      // rank 0: the row's bins
   u64 g_mass[kBins];
-  u64 cand[kCand], sorted[kCand];  // rank 0: tokens of the cut's bin
+  // rank 0: the list, in order of arrival, then ranked (by key, later by index)
+  __align__(16) u64 cand[kCand];
+  u64 sorted[kCand];
+  __align__(16) uint32_t place[kCand];
   u64 warp_mass[kWarps], warp_best[kWarps];
   uint32_t warp_cnt[kWarps];
   u64 best, mass;   // this CTA's largest key, kept mass
@@ -67,22 +74,47 @@ __device__ __forceinline__ float order_value(uint32_t o) {
 __device__ __forceinline__ u64 token_key(float v, int i) {
   return ((u64)order_bits(v) << 32) | (uint32_t)~(uint32_t)i;
 }
-// floor(f * m) for f in [0, 1)
+// floor(f * m) for f in [0, 1), or its ceiling
 __device__ __forceinline__ u64 fraction_of(float f, u64 m, bool up) {
   const u64 fix = (u64)((double)f * 18446744073709551616.0);  // exact down to 2^-40
   return __umul64hi(fix, m) + (up && fix * m != 0 ? 1 : 0);
 }
 
 struct Weights {
-  float top;        // the row's largest logit
-  double inv_t, scale;
-  // w of a logit that is not NaN
-  __device__ __forceinline__ double w(float x) const {
-    if (top == INFINITY) return x == INFINITY ? 1.0 : 0.0;
+  float top;           // the row's largest logit
+  double octaves;      // 64 log2(e) / T: (x - top) in 64ths of an octave
+  double scale;        // mass of w = 1
+  int mass_bits;       // its power of two
+  const double *table;
+
+  // w of a logit that is not NaN, to 2^-44: with y = 64 log2 w split into an
+  // integer k and |f| <= 1/2, w = 2^(k >> 6) 2^((k & 63) / 64) e^r for r = f ln2 / 64,
+  // e^r by its series to r^4 (r^5 / 120 < 2^-44).  (Table look-up and a short
+  // series: P. T. P. Tang, ACM TOMS 15(2), 1989.)
+  __device__ __forceinline__ double w(float x) const { return w_scaled(x, 0); }
+  // w 2^bits
+  __device__ __forceinline__ double w_scaled(float x, int bits) const {
+    if (top == INFINITY) return x == INFINITY ? (bits ? scale : 1.0) : 0.0;
     if (x == -INFINITY) return 0.0;
-    return exp(((double)x - (double)top) * inv_t);
+    constexpr double kMagic = 6755399441055744.0;  // 1.5 2^52: the sum's low word is round(y)
+    constexpr double kC = 0.010830424696249145;    // ln2 / 64
+    const double y = fmax(((double)x - (double)top) * octaves, -60000.0);
+    const double kd = y + kMagic;
+    const int k = __double2loint(kd);
+    const double f = y - (kd - kMagic);
+    double e = fma(f, kC * kC * kC * kC / 24, kC * kC * kC / 6);
+    e = fma(f, e, kC * kC / 2);
+    e = fma(f, e, kC);
+    e *= f;
+    const double t = table[k & 63];
+    const double v = fma(t, e, t);
+    return __hiloint2double(__double2hiint(v) + (((k >> 6) + bits) << 20), __double2loint(v));
   }
-  __device__ __forceinline__ u64 mass(double w) const { return __double2ull_rn(w * scale); }
+  // round(w 2^mass_bits), below 2^51
+  __device__ __forceinline__ u64 mass(float x) const {
+    const double v = w_scaled(x, mass_bits) + 4503599627370496.0;  // 2^52
+    return (u64)__double_as_longlong(v) & 0xFFFFFFFFFFFFFull;
+  }
 };
 
 __device__ __forceinline__ u64 warp_sum64(u64 v) {
@@ -90,17 +122,50 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// inclusive sums over the lanes
+__device__ __forceinline__ u64 warp_scan64(u64 v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
+// the exclusive sum of the lanes' (= warps') values before this warp's, and their total
+__device__ __forceinline__ u64 before_warp(const u64 *v, u64 &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const u64 in = warp_scan64(v[lane]);
+  total = __shfl_sync(0xffffffffu, in, 31);
+  return __shfl_sync(0xffffffffu, in, warp) - v[warp];
+}
+static_assert(kWarps == 32, "a lane per warp");
 
 struct Row {
   cg::cluster_group cl;
   Shared &s;
   const float *x;  // the slice: shared memory, or the row in global memory
   int base, len;   // the slice's first token and length
-  int w0, w1;      // this warp's stretch of the slice
   int rank, ctas;
 
-  __device__ __forceinline__ void clear_bins() {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.cnt[i] = s.lo[i] = s.hi[i] = 0;
+  template <class F>
+  __device__ __forceinline__ void each(F f) {
+    int i = threadIdx.x;
+    for (; i + 3 * kThreads < len; i += 4 * kThreads) {
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = x[i + k * kThreads];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f(v[k], i + k * kThreads);
+    }
+    for (; i < len; i += kThreads) f(x[i], i);
+  }
+  __device__ __forceinline__ void clear_bins(bool masses) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+      s.cnt[i] = 0;
+      s.lo[i] = 0;
+      if (masses) s.hi[i] = 0;
+    }
     if (rank == 0 && threadIdx.x == 0) s.n_cand = 0;
     __syncthreads();
   }
@@ -119,21 +184,29 @@ struct Row {
   // what lies above the bins.  The result lands in every CTA's s.bin (-1: never
   // reached), s.bin_cnt, s.above_*.
   __device__ void find(uint32_t k, float top_p, uint32_t first_cnt, u64 first_mass) {
-    cl.sync();  // every CTA's bins are complete
+    if (ctas > 1)
+      cl.sync();  // every CTA's bins are complete
+    else
+      __syncthreads();
     const int per = kBins / ctas;
     for (int i = threadIdx.x; i < per; i += kThreads) {
       const int bin = rank * per + i;
       uint32_t c = 0;
       u64 m = 0;
+#pragma unroll 4
       for (int r = 0; r < ctas; ++r) {
         c += *cl.map_shared_rank(&s.cnt[bin], r);
-        m += (u64)*cl.map_shared_rank(&s.lo[bin], r) +
-             ((u64)*cl.map_shared_rank(&s.hi[bin], r) << 32);
+        if (!k)
+          m += (u64)*cl.map_shared_rank(&s.lo[bin], r) +
+               ((u64)*cl.map_shared_rank(&s.hi[bin], r) << 32);
       }
       *cl.map_shared_rank(&s.g_cnt[bin], 0) = c;
       *cl.map_shared_rank(&s.g_mass[bin], 0) = m;
     }
-    cl.sync();
+    if (ctas > 1)
+      cl.sync();
+    else
+      __syncthreads();
     if (rank == 0) {
       const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
       constexpr int kPer = kBins / kThreads;
@@ -147,35 +220,30 @@ struct Row {
         msum += m[i];
       }
       uint32_t cin = csum;
-      u64 min_ = msum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t cu = __shfl_up_sync(0xffffffffu, cin, o);
-        const u64 mu = __shfl_up_sync(0xffffffffu, min_, o);
-        if (lane >= o) {
-          cin += cu;
-          min_ += mu;
-        }
+        if (lane >= o) cin += cu;
       }
+      const u64 min_ = warp_scan64(msum);
       if (lane == 31) {
         s.warp_cnt[warp] = cin;
         s.warp_mass[warp] = min_;
       }
       if (threadIdx.x == 0) s.bin = -1;
       __syncthreads();
-      uint32_t cb = first_cnt;
-      u64 mb = first_mass, total = first_mass;
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) {
-          cb += s.warp_cnt[w];
-          mb += s.warp_mass[w];
-        }
-        total += s.warp_mass[w];
+      u64 total;
+      u64 mb = first_mass + before_warp(s.warp_mass, total) + min_ - msum;
+      total += first_mass;
+      uint32_t cw = s.warp_cnt[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t cu = __shfl_up_sync(0xffffffffu, cw, o);
+        if (lane >= o) cw += cu;
       }
+      uint32_t cb = first_cnt + __shfl_sync(0xffffffffu, cw, warp) - s.warp_cnt[warp] + cin - csum;
       u64 target = s.target;
       if (top_p == top_p) target = max(fraction_of(fmaxf(top_p, 0.f), total, true), 1ull);
-      cb += cin - csum;
-      mb += min_ - msum;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const bool here = k ? (cb < k && cb + c[i] >= k) : (mb < target && mb + m[i] >= target);
@@ -199,29 +267,67 @@ struct Row {
         o->target = s.target;
       }
     }
-    cl.sync();
+    if (ctas > 1)
+      cl.sync();
+    else
+      __syncthreads();
+  }
+
+  // tokens of `pred` into rank 0's list, in any order
+  template <class P>
+  __device__ __forceinline__ void gather(P pred) {
+    int *n_cand = cl.map_shared_rank(&s.n_cand, 0);
+    u64 *cand = cl.map_shared_rank(&s.cand[0], 0);
+    each([&](float v, int i) {
+      const u64 key = token_key(v, base + i);
+      if (pred(v, key)) cand[atomicAdd(n_cand, 1)] = key;
+    });
+    if (ctas > 1)
+      cl.sync();
+    else
+      __syncthreads();
+  }
+
+  // rank 0: the list in order of falling keys into s.sorted.  A token's place is
+  // the number of larger keys, counted by as many threads as the block has to spare.
+  __device__ void rank_list(int n) {
+    int share = 1;
+    while (2 * share * n <= kThreads) share *= 2;
+    for (int i = threadIdx.x; i < n; i += kThreads) s.place[i] = 0;
+    __syncthreads();
+    for (int t = threadIdx.x; t < n * share; t += kThreads) {
+      const int i = t / share, j0 = t - i * share;
+      const u64 key = s.cand[i];
+      uint32_t c = 0;
+#pragma unroll 4
+      for (int j = j0; j < n; j += share) c += s.cand[j] > key;
+      if (c) atomicAdd(&s.place[i], c);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) s.sorted[s.place[i]] = s.cand[i];
+    __syncthreads();
   }
 
   // The cut of the first k tokens (k > 0) or of the shortest prefix that holds
   // the top_p share of the mass, among the keys >= `within`: every CTA
-  // returns the key of the last kept token.
-  __device__ u64 cut(uint32_t k, float top_p, u64 within, const Weights &W, float bin_scale) {
+  // returns the key of the last kept token.  Where `listed` is given and the tokens
+  // down to the cut's bin fit the list, they are left there instead (*listed set).
+  __device__ u64 cut(uint32_t k, float top_p, u64 within, const Weights &W, float bin_scale,
+                     bool *listed) {
     auto value_bin = [&](float v) {
       if (v == W.top) return 0;
       return (int)fminf((W.top - v) * bin_scale, (float)(kBins - 1));
     };
-    clear_bins();
+    clear_bins(!k);
     {
       // the last bin also takes all that lies below the range: summed in
       // registers first, as half the row may fall there
       uint32_t rest_n = 0;
       u64 rest_m = 0;
-#pragma unroll 4
-      for (int i = threadIdx.x; i < len; i += kThreads) {
-        const float v = x[i];
+      each([&](float v, int i) {
         const u64 key = token_key(v, base + i);
-        if (key < within) continue;
-        const u64 m = k ? 0 : W.mass(W.w(v));
+        if (key < within) return;
+        const u64 m = k ? 0 : W.mass(v);
         const int bin = value_bin(v);
         if (bin < kBins - 1) {
           add(bin, 1, m);
@@ -229,7 +335,7 @@ struct Row {
           ++rest_n;
           rest_m += m;
         }
-      }
+      });
       rest_n = __reduce_add_sync(0xffffffffu, rest_n);
       rest_m = warp_sum64(rest_m);
       if ((threadIdx.x & 31) == 0) add(kBins - 1, rest_n, rest_m);
@@ -237,6 +343,11 @@ struct Row {
     find(k, top_p, 0, 0);
     if (s.bin < 0) return within;  // fewer than k tokens: all of them
     const int vbin = s.bin;
+    if (listed && s.above_cnt + s.bin_cnt <= kCand) {
+      *listed = true;
+      gather([&](float v, u64 key) { return key >= within && value_bin(v) <= vbin; });
+      return within;
+    }
     // narrow a crowded bin by digits of the key, highest first
     int shift = 64, bits = 0;
     u64 prefix = 0;
@@ -247,36 +358,21 @@ struct Row {
       bits = min(11, shift);
       const uint32_t above_cnt = s.above_cnt;
       const u64 above_mass = s.above_mass;
-      clear_bins();
-      for (int i = threadIdx.x; i < len; i += kThreads) {
-        const float v = x[i];
+      clear_bins(!k);
+      each([&](float v, int i) {
         const u64 key = token_key(v, base + i);
-        if (!inside(v, key)) continue;
+        if (!inside(v, key)) return;
         const int digit = (int)((key >> (shift - bits)) & ((1u << bits) - 1));
-        add((1 << bits) - 1 - digit, 1, k ? 0 : W.mass(W.w(v)));
-      }
+        add((1 << bits) - 1 - digit, 1, k ? 0 : W.mass(v));
+      });
       find(k, NAN, above_cnt, above_mass);
       prefix = (prefix << bits) | (u64)((1 << bits) - 1 - s.bin);
       shift -= bits;
     }
-    // the bin's tokens into rank 0's list, in any order
-    int *n_cand = cl.map_shared_rank(&s.n_cand, 0);
-    u64 *cand = cl.map_shared_rank(&s.cand[0], 0);
-    for (int i = threadIdx.x; i < len; i += kThreads) {
-      const float v = x[i];
-      const u64 key = token_key(v, base + i);
-      if (inside(v, key)) cand[atomicAdd(n_cand, 1)] = key;
-    }
-    cl.sync();
+    gather(inside);
     if (rank == 0) {
       const int n = s.n_cand;
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const u64 key = s.cand[i];
-        int place = 0;
-        for (int j = 0; j < n; ++j) place += s.cand[j] > key;
-        s.sorted[place] = key;
-      }
-      __syncthreads();
+      rank_list(n);
       if (k) {
         if (threadIdx.x == 0) s.cut = s.sorted[k - s.above_cnt - 1];
       } else if (threadIdx.x < 32) {
@@ -285,12 +381,8 @@ struct Row {
         u64 found = s.sorted[n - 1];
         for (int i0 = 0; i0 < n; i0 += 32) {
           const int i = i0 + threadIdx.x;
-          u64 m = i < n ? W.mass(W.w(order_value((uint32_t)(s.sorted[i] >> 32)))) : 0;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const u64 up = __shfl_up_sync(0xffffffffu, m, o);
-            if ((int)threadIdx.x >= o) m += up;
-          }
+          const u64 m =
+              warp_scan64(i < n ? W.mass(order_value((uint32_t)(s.sorted[i] >> 32))) : 0);
           const uint32_t hit = __ballot_sync(0xffffffffu, i < n && run + m >= s.target);
           if (hit) {
             found = s.sorted[i0 + __ffs(hit) - 1];
@@ -303,17 +395,65 @@ struct Row {
       __syncthreads();
       if (threadIdx.x > 0 && threadIdx.x < ctas) cl.map_shared_rank(&s, threadIdx.x)->cut = s.cut;
     }
-    cl.sync();
+    if (ctas > 1)
+      cl.sync();
+    else
+      __syncthreads();
     return s.cut;
+  }
+
+  // rank 0: both cuts and the draw on the list.  top_p_target: the mass the top-p
+  // prefix has to reach, or 0 to take the share of the first k tokens' mass.
+  __device__ void draw_listed(uint32_t k, float top_p, u64 top_p_target, double min_w, float u,
+                              const Weights &W, int32_t *token, float *prob) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = threadIdx.x;
+    const int n = s.n_cand;
+    rank_list(n);
+    const int n_k = k ? min(n, (int)k) : n;
+    const u64 key = i < n_k ? s.sorted[i] : 0;
+    const float v = order_value((uint32_t)(key >> 32));
+    const u64 m = i < n_k ? W.mass(v) : 0;
+    u64 in = warp_scan64(m), total;
+    if (lane == 31) s.warp_mass[warp] = in;
+    __syncthreads();
+    in += before_warp(s.warp_mass, total);
+    if (!top_p_target && top_p < 1.f)
+      top_p_target = max(fraction_of(fmaxf(top_p, 0.f), total, true), 1ull);
+    // the kept ones are the first of the ranked ones
+    const bool keep = i < n_k && (!top_p_target || in - m < top_p_target) && W.w(v) >= min_w;
+    const int n_keep = __syncthreads_count(keep);
+    if (keep) {  // ranked again, by index: the low word of a key is ~index
+      s.cand[i] = (key << 32) | (uint32_t)i;
+      s.g_mass[i] = m;
+    }
+    __syncthreads();
+    rank_list(n_keep);
+    const uint32_t at = i < n_keep ? (uint32_t)s.sorted[i] & (kCand - 1) : 0;
+    const u64 mine = i < n_keep ? s.g_mass[at] : 0;
+    in = warp_scan64(mine);
+    if (lane == 31) s.warp_mass[warp] = in;
+    __syncthreads();
+    in += before_warp(s.warp_mass, total);
+    const u64 point = fraction_of(u, total, false);
+    if (in > point && in - mine <= point) {  // one thread: its mass is not 0
+      const uint32_t index = ~(uint32_t)(s.sorted[i] >> 32);
+      *token = (int32_t)index;
+      if (prob) s.target = at;
+    }
+    if (prob) {  // w itself over the kept mass
+      __syncthreads();
+      if (i == (int)s.target) *prob = (float)(W.w_scaled(v, W.mass_bits) / (double)total);
+    }
   }
 };
 
-__global__ void __launch_bounds__(kThreads) sample_kernel(
+__global__ void __launch_bounds__(kThreads, 1) sample_kernel(
     const float *logits, int n, long long row_stride, int slice, int resident, int mass_bits,
     const mlm_sample_params *params, const float *uniform, int32_t *token, float *prob) {
   extern __shared__ __align__(16) uint8_t s_raw[];
   Shared &s = *reinterpret_cast<Shared *>(s_raw);
   float *s_x = reinterpret_cast<float *>(s_raw + sizeof(Shared));
+  if (threadIdx.x < 64) s.exp2_64[threadIdx.x] = exp2(threadIdx.x / 64.0);
   pdl_wait_then_release();
   cg::cluster_group cl = cg::this_cluster();
   const int rank = cl.block_rank(), ctas = cl.num_blocks();
@@ -321,32 +461,32 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int base = min(n, rank * slice), len = min(n - base, slice);
   const float *g = logits + row * row_stride + base;
-  const int per = (len + kWarps * 32 - 1) / (kWarps * 32) * 32;
-  Row r{cl, s, resident ? s_x : g, base, len, min(len, warp * per), min(len, (warp + 1) * per),
-        rank, ctas};
+  const mlm_sample_params p = params[row];
+  Row r{cl, s, g, base, len, rank, ctas};
 
   // the slice into shared memory; the row's largest key
   u64 best = 0;
-#pragma unroll 8
-  for (int i = threadIdx.x; i < len; i += kThreads) {
-    const float v = g[i];
+  r.each([&](float v, int i) {
     if (resident) s_x[i] = v;
     const u64 key = token_key(v, base + i);
     best = key > best ? key : best;
-  }
+  });
+  if (resident) r.x = s_x;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   if (lane == 0) s.warp_best[warp] = best;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kWarps; ++w) best = max(best, s.warp_best[w]);
-    s.best = best;
+  best = s.warp_best[lane];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if (ctas > 1) {
+    if (threadIdx.x == 0) s.best = best;
+    cl.sync();
+    best = *cl.map_shared_rank(&s.best, lane < ctas ? lane : 0);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   }
-  cl.sync();
-  best = 0;
-  for (int q = 0; q < ctas; ++q) best = max(best, *cl.map_shared_rank(&s.best, q));
 
-  const mlm_sample_params p = params[row];
   const float top = order_value((uint32_t)(best >> 32));
   const bool none = best < kAll || top == -INFINITY;
   if (none || !(p.temperature > 0.f)) {
@@ -360,78 +500,110 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(
   }
   Weights W;
   W.top = top;
-  W.inv_t = 1.0 / (double)p.temperature;
+  W.octaves = 92.332482616893656 / (double)p.temperature;  // 64 log2(e) / T
   W.scale = (double)(1ull << mass_bits);
-  u64 cut = kAll;
+  W.mass_bits = mass_bits;
+  W.table = s.exp2_64;
   // bins over the logits that matter: 24 temperatures, but at least 16 and at
   // most 64 below the largest
   const float bin_scale = (float)kBins / fminf(fmaxf(24.f * p.temperature, 16.f), 64.f);
-  if (p.top_k > 0 && p.top_k < n) cut = r.cut((uint32_t)p.top_k, NAN, cut, W, bin_scale);
-  if (p.top_p < 1.f) cut = r.cut(0, p.top_p, cut, W, bin_scale);
-
-  // the kept mass of every warp's stretch
+  const uint32_t k = p.top_k > 0 && p.top_k < n ? (uint32_t)p.top_k : 0;
   const double min_w = p.min_p > 0.f ? fmin((double)p.min_p, 1.0) : 0.0;
-  auto kept = [&](int i) -> u64 {
-    const float v = r.x[i];
-    if (token_key(v, base + i) < cut) return 0;
-    const double w = W.w(v);
-    return w >= min_w ? W.mass(w) : 0;
-  };
-  u64 m = 0;
-#pragma unroll 4
-  for (int i = r.w0 + lane; i < r.w1; i += 32) m += kept(i);
-  m = warp_sum64(m);
-  if (lane == 0) s.warp_mass[warp] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    u64 t = 0;
-    for (int w = 0; w < kWarps; ++w) t += s.warp_mass[w];
-    s.mass = t;
-  }
-  cl.sync();
-  u64 before = 0, total = 0;
-  for (int q = 0; q < ctas; ++q) {
-    const u64 t = *cl.map_shared_rank(&s.mass, q);
-    if (q < rank) before += t;
-    total += t;
-  }
   float u = uniform[row];
   u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;  // NaN: 0
-  const u64 point = fraction_of(u, total, false);  // the first token whose running mass exceeds it
-  for (int w = 0; w < warp; ++w) before += s.warp_mass[w];
-  if (point >= before && point < before + m) {
-    u64 run = before;
-    for (int i0 = r.w0; i0 < r.w1; i0 += 32) {
-      const int i = i0 + lane;
-      u64 t = i < r.w1 ? kept(i) : 0;
+  u64 cut = kAll;
+  bool listed = false;
+  if (k) cut = r.cut(k, NAN, cut, W, bin_scale, &listed);
+  if (p.top_p < 1.f && !listed) cut = r.cut(0, p.top_p, cut, W, bin_scale, k ? nullptr : &listed);
+  if (listed) {
+    if (rank == 0)
+      r.draw_listed(k, p.top_p, k ? 0 : s.target, min_w, u, W, token + row, prob ? prob + row : nullptr);
+    return;  // the other CTAs' shared memory is no longer read (gather ended in a barrier)
+  }
+
+  // the kept mass of every warp's stretch
+  auto kept = [&](float v, int i) -> u64 {
+    if (token_key(v, base + i) < cut) return 0;
+    return min_w == 0.0 || W.w(v) >= min_w ? W.mass(v) : 0;
+  };
+  // this warp's share of a range, 4 loads in flight
+  auto range_mass = [&](int i0, int i1) -> u64 {
+    u64 m = 0;
+    int i = i0 + lane;
+    for (; i + 96 < i1; i += 128) {
+      float v[4];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 up = __shfl_up_sync(0xffffffffu, t, o);
-        if (lane >= o) t += up;
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, run + t > point);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
-          token[row] = base + i;
-          if (prob) prob[row] = (float)(W.w(r.x[i]) * W.scale / (double)total);
+      for (int j = 0; j < 4; ++j) v[j] = r.x[i + 32 * j];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m += kept(v[j], i + 32 * j);
+    }
+    for (; i < i1; i += 32) m += kept(r.x[i], i);
+    return warp_sum64(m);
+  };
+  const int per = (len + kWarps * 32 - 1) / (kWarps * 32) * 32;
+  u64 m = range_mass(min(len, warp * per), min(len, (warp + 1) * per));
+  if (lane == 0) s.warp_mass[warp] = m;
+  __syncthreads();
+  u64 total;
+  u64 before = before_warp(s.warp_mass, total);
+  if (ctas > 1) {
+    if (threadIdx.x == 0) s.mass = total;
+    cl.sync();
+    const u64 of = lane < ctas ? *cl.map_shared_rank(&s.mass, lane) : 0;
+    const u64 in = warp_scan64(of);
+    total = __shfl_sync(0xffffffffu, in, 31);
+    before += __shfl_sync(0xffffffffu, in - of, rank);
+  }
+  const u64 point = fraction_of(u, total, false);  // the first token whose running mass exceeds it
+  // the stretch that holds the point, 1/32 of it per warp, then 32 tokens at a time
+  if (threadIdx.x == 0) s.bin = -1;
+  __syncthreads();
+  if (lane == 0 && point >= before && point < before + m) {
+    s.bin = warp;
+    s.target = before;
+  }
+  __syncthreads();
+  if (s.bin >= 0) {
+    const int a0 = min(len, s.bin * per), a1 = min(len, a0 + per);
+    const int sub = (per + kWarps * 32 - 1) / (kWarps * 32) * 32;
+    const int b0 = min(a1, a0 + warp * sub), b1 = min(a1, b0 + sub);
+    before = s.target;
+    m = range_mass(b0, b1);
+    if (lane == 0) s.warp_mass[warp] = m;
+    __syncthreads();
+    u64 unused;
+    before += before_warp(s.warp_mass, unused);
+    if (point >= before && point < before + m) {
+      for (int i0 = b0; i0 < b1; i0 += 32) {
+        const int i = i0 + lane;
+        const u64 t = warp_scan64(i < b1 ? kept(r.x[i], i) : 0);
+        const uint32_t hit = __ballot_sync(0xffffffffu, before + t > point);
+        if (hit) {
+          if (lane == __ffs(hit) - 1) {
+            token[row] = base + i;
+            if (prob) prob[row] = (float)(W.w_scaled(r.x[i], mass_bits) / (double)total);
+          }
+          break;
         }
-        break;
+        before += __shfl_sync(0xffffffffu, t, 31);
       }
-      run += __shfl_sync(0xffffffffu, t, 31);
     }
   }
-  cl.sync();  // no CTA leaves while another may still read its s.mass
+  if (ctas > 1) cl.sync();  // no CTA leaves while another may still read its s.mass
 }
 
 constexpr int kMaxN = 1 << 22;
 // shared memory a slice may take beside the bins (one CTA per SM)
-constexpr size_t kSliceBytes = 160 * 1024;
+constexpr size_t kSliceBytes = 150 * 1024;
+static_assert(sizeof(Shared) + kSliceBytes <= 227 * 1024, "a CTA's shared memory");
 
 }  // namespace
 
 int sample_init(mlm_ctx *ctx) {
   MLM_CUDA_TRY(ctx, cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)(sizeof(Shared) + kSliceBytes)));
+  MLM_CUDA_TRY(ctx, cudaFuncSetAttribute(sample_kernel,
+                                         cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   return MLM_OK;
 }
 
@@ -453,7 +625,7 @@ extern "C" int mlm_sample_f32(mlm_ctx *ctx, const float *logits, int rows, int n
               MLM_ERR_ALIGN, "mlm_sample_f32: buffers must be 4-byte aligned");
   DeviceGuard guard(ctx);
   int ctas = kMaxCluster;
-  while (ctas > 1 && (rows * ctas > ctx->sm_count || n < 2048 * ctas)) ctas /= 2;
+  while (ctas > 1 && (rows * ctas > ctx->sm_count || n < kMinSlice * ctas)) ctas /= 2;
   const int slice = (n + ctas - 1) / ctas;
   const int resident = (size_t)slice * 4 <= kSliceBytes;
   int bits = 62;
