@@ -693,8 +693,8 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
 // per SM beside the warps' head pieces
 template <int NT, bool DUP>
 struct FewShape {
-  static constexpr int warps = DUP ? 16 : NT == 1 ? 14 : 8;
-  static constexpr int stages = NT == 1 ? 2 : 3;
+  static constexpr int warps = DUP ? 16 : NT == 1 ? 14 : 12;
+  static constexpr int stages = 2;
   static constexpr int cols = DUP ? 4 : 8 * NT;
   static constexpr size_t smem(int batch) {
     return (size_t)warps * stages * kStage + (size_t)warps * cols * kPieceRow * 4 +

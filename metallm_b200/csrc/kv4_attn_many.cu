@@ -13,10 +13,10 @@
 //   - 4 warps per row tile do the softmax, a thread per row: S from TMEM, the
 //     weights back as fp16 over it, where the second product reads them as its A
 //     operand.
-// The running maximum follows only when a score leads it by more than 2^8 (a
-// weight is then at most 2^8, an fp16 value), so the accumulator in TMEM is
-// rescaled once in a row's life, as a rule.  Scores, maxima and sums are fp32;
-// K, V and the weights are fp16 operands.
+// The running maximum follows only when a score leads it by more than 2^14 (a
+// weight is then still an fp16 value of full precision), so the accumulator in
+// TMEM is rescaled once in a row's life, as a rule.  Scores, maxima and sums are
+// fp32; K, V and the weights are fp16 operands.
 //
 // V^T is the N-major B operand of the second product: both K and V lie in
 // shared memory as [key][dimension] in the 128-byte swizzle, the eight
@@ -53,9 +53,9 @@ constexpr int kOffTmem = kOffBar + 8 * kBars;
 constexpr int kOffLine = kOffTmem + 16;     // [batch + 1] 64-bit offsets
 constexpr size_t smem_bytes(int batch) { return kOffLine + 8 * (size_t)(batch + 1); }
 constexpr int kTmemCols = 512;  // S/P of tile 0 and 1, O of tile 0 and 1
-constexpr int kPartRow = kKv4D + 4;  // a row of a part: o[128], m, l, padding
+constexpr int kPartFloats = kRows * (kKv4D + 2);  // o, then m and l
 constexpr float kScale2 = kInvSqrtD * kLog2e;
-constexpr float kLead = 8.f / kScale2;
+constexpr float kLead = 14.f / kScale2;
 
 // instruction descriptors: fp16 A and B, fp32 accumulators, M = N = 128; B K-major
 // (S = Q K^T) or N-major (O = P V)
@@ -101,18 +101,38 @@ __device__ __forceinline__ void commit(uint32_t bar) {
 __device__ __forceinline__ void arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// 32 columns of the warp's lanes; the values are there after tmem_wait_ld, which
+// names them so that no use moves above it
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-      "tcgen05.wait::ld.sync.aligned;"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
         "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
         "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
         "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
         "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]),
+                 "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
+                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]),
+                 "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                 "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29])
+               :
+               : "memory");
+  asm volatile("" : "+r"(v[30]), "+r"(v[31])::"memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *v) {
@@ -298,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
   __syncthreads();
   const uint32_t tmem = *tmem_slot;
   const long long total = s_off[a.batch];
-  const long long quota = max(4ll, (total + gridDim.x - 1) / gridDim.x);
+  const long long quota = max(1ll, (total + gridDim.x - 1) / gridDim.x);
   const long long x0 = min(total, blockIdx.x * quota), x1 = min(total, x0 + quota);
   if (blockIdx.x == 0) {  // the cut, for the joining kernel
     long long *plan = reinterpret_cast<long long *>(a.plan);
@@ -331,20 +351,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
       const int seen = mine ? max(0, p.len - p.count + tok + 1) : 0;
       const size_t at = (((size_t)p.b * a.tokens + tok) * a.n_heads + p.h * a.group +
                          (row - tok * a.group)) * kKv4D;
-      // the row's q, in the order of the codes
-      {
-        const uint4 *src = reinterpret_cast<const uint4 *>(a.q + at);
+      // Q in the order of the codes: half a warp per row
+      uint8_t *s_q = smem + tile * kOperand;
+      auto row_at = [&](int i) {  // where row i of the warp's 32 lies in q and out
+        return ((uint64_t)__shfl_sync(0xffffffffu, (uint32_t)(at >> 32), i) << 32) |
+               __shfl_sync(0xffffffffu, (uint32_t)at, i);
+      };
+      const uint32_t rows = __ballot_sync(0xffffffffu, mine);
+      const int r0 = (warp & 3) * 32;
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const uint4 v = mine ? src[c] : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4 *>(smem + tile * kOperand + chunk_at(r, c)) =
-              make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
-                         __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        tc_fence_before();
-        arrive(bar + 8 * kQfull);
+      for (int i = 0; i < 16; ++i) {
+        const int j = 2 * i + (lane >> 4), c = lane & 15;
+        const uint64_t from = row_at(j);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if ((rows >> j) & 1) v = *reinterpret_cast<const uint4 *>(a.q + from + 8 * c);
+        *reinterpret_cast<uint4 *>(s_q + chunk_at(r0 + j, c)) =
+            make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                       __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc_fence_before();
+      arrive(bar + 8 * kQfull);
       if (tile * kTile >= live) {  // no row of this tile: its products do not run
         // not past the other tile: its arrivals for this item come first
         ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar + 8 * kQfull, n_q++ & 1, a.status));
@@ -360,62 +387,84 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
         ++n_s;
         tc_fence_after();
         const int lim = seen - kt * kTile;  // keys of the tile that the row sees
-        uint32_t w[64];
-        uint64_t sum = 0;
-        // weights against the maximum m; returns the tile's largest score
         auto weights = [&](auto mask_tag) {
           constexpr bool MASK = decltype(mask_tag)::value;
-          const float m2 = m == -INFINITY ? 0.f : -m * kScale2;
-          const uint64_t mm = pair(m2, m2), cc = pair(kScale2, kScale2);
-          float top0 = -INFINITY, top1 = -INFINITY;
-          sum = 0;
+          uint32_t s[2][32];
+          float m2 = m == -INFINITY ? 0.f : -m * kScale2;
+          tmem_ld32(ts, s[0]);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t s[32];
-            tmem_ld32(ts + 32 * c, s);
+            uint32_t(&v)[32] = s[c & 1];
+            tmem_wait_ld(v);
+            if (c < 3) tmem_ld32(ts + 32 * (c + 1), s[(c + 1) & 1]);
+            float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
-              float s0 = __uint_as_float(s[k]), s1 = __uint_as_float(s[k + 1]);
               if (MASK) {
-                if (32 * c + k >= lim) s0 = -INFINITY;
-                if (32 * c + k + 1 >= lim) s1 = -INFINITY;
+                if (32 * c + k >= lim) v[k] = 0xFF800000u;
+                if (32 * c + k + 1 >= lim) v[k + 1] = 0xFF800000u;
               }
-              top0 = fmaxf(top0, s0);
-              top1 = fmaxf(top1, s1);
-              const float2 e = unpair(fma2(pair(s0, s1), cc, mm));
-              const float p0 = ex2(e.x), p1 = ex2(e.y);
-              sum = add2(sum, pair(p0, p1));
-              w[16 * c + k / 2] = pack_f16(p0, p1);
+              top = fmaxf(top, __uint_as_float(v[k]));
+              top1 = fmaxf(top1, __uint_as_float(v[k + 1]));
             }
-          }
-          return fmaxf(top0, top1);
-        };
-        const bool masked = __any_sync(0xffffffffu, lim < kTile);
-        const float top = masked ? weights(std::true_type()) : weights(std::false_type());
-        if (__any_sync(0xffffffffu, top > m + kLead)) {
-          const float up = fmaxf(m, top);
-          const float f = up == m ? 1.f : ex2((m - up) * kScale2);
-          if (kt > p.kt0) {
+            top = fmaxf(top, top1);
+            if (__any_sync(0xffffffffu, top > m + kLead)) {
+              // a new maximum: what has been summed against the old one is scaled,
+              // O, l and this tile's weights so far
+              if (c < 3) tmem_wait_ld(s[(c + 1) & 1]);
+              const float up = fmaxf(m, top);
+              const float f = up == m ? 1.f : ex2((m - up) * kScale2);
+              if (kt > p.kt0) {
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t o[32];
-              tmem_ld32(to + 32 * c, o);
+                for (int j = 0; j < 4; ++j) {
+                  uint32_t o[32];
+                  tmem_ld32(to + 32 * j, o);
+                  tmem_wait_ld(o);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              tmem_st32(to + 32 * c, o);
+                  for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                  tmem_st32(to + 32 * j, o);
+                }
+              }
+              tmem_wait_st();
+#pragma unroll 1
+              for (int j = 0; j < (c + 1) / 2; ++j) {  // 64 weights at a time
+                uint32_t o[32];
+                tmem_ld32(ts + 32 * j, o);
+                tmem_wait_ld(o);
+                uint32_t h[16];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                  for (int k = 0; k < 16; ++k) {
+                    const float2 e = unpack_f16(o[16 * half + k]);
+                    h[k] = pack_f16(e.x * f, e.y * f);
+                  }
+                  if (2 * j + half < c) tmem_st16(ts + 32 * j + 16 * half, h);
+                }
+              }
+              tmem_wait_st();
+              const float2 l = unpair(l2);
+              l2 = pair(l.x * f, l.y * f);
+              m = up;
+              m2 = m == -INFINITY ? 0.f : -m * kScale2;
             }
+            const uint64_t mm = pair(m2, m2), cc = pair(kScale2, kScale2);
+            uint32_t w[16];
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+              const float2 e =
+                  unpair(fma2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), cc, mm));
+              const float p0 = ex2(e.x), p1 = ex2(e.y);
+              l2 = add2(l2, pair(p0, p1));
+              w[k / 2] = pack_f16(p0, p1);
+            }
+            tmem_st16(ts + 16 * c, w);  // over scores that have been read
           }
-          const float2 l = unpair(l2);
-          l2 = pair(l.x * f, l.y * f);
-          m = up;
-          if (masked)
-            weights(std::true_type());
-          else
-            weights(std::false_type());
-        }
-        l2 = add2(l2, sum);
-        tmem_st32(ts, w);
-        tmem_st32(ts + 32, w + 32);
+        };
+        if (__any_sync(0xffffffffu, lim < kTile))
+          weights(std::true_type());
+        else
+          weights(std::false_type());
         tmem_wait_st();
         tc_fence_before();
         arrive(bar + 8 * (kPfull + tile));
@@ -431,36 +480,45 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
       const long long item = walk.x - p.kt1;  // the item's first tile on the line
       const bool whole = p.kt0 == 0 && p.kt1 == p.nkt;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      float *part = a.parts + (((size_t)blockIdx.x * 2 + (item < x0 ? 0 : 1)) * kRows +
-                               tile * kTile + r) * kPartRow;
+      // parts: [4 columns][row], then the rows' maxima and sums
+      float *part = a.parts + ((size_t)blockIdx.x * 2 + (item < x0 ? 0 : 1)) * kPartFloats;
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
         tmem_ld32(to + 32 * c, o);
-        if (mine) {
+        tmem_wait_ld(o);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float e[8];  // columns 0 4 1 5 2 6 3 7 back in order
+        for (int j = 0; j < 4; ++j) {
+          float e[8];  // columns 0 4 1 5 2 6 3 7 back in order
 #pragma unroll
-            for (int k = 0; k < 8; ++k) e[(k >> 1) + 4 * (k & 1)] = __uint_as_float(o[8 * j + k]);
-            if (whole) {
-              OutT h[8];
+          for (int k = 0; k < 8; ++k) e[(k >> 1) + 4 * (k & 1)] = __uint_as_float(o[8 * j + k]);
+          if (whole) {  // by way of Q's place, which no product reads any more
+            OutT h[8];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) h[k] = from_float<OutT>(e[k] * inv);
-              *reinterpret_cast<uint4 *>(reinterpret_cast<OutT *>(a.out) + at + 32 * c + 8 * j) =
-                  *reinterpret_cast<const uint4 *>(h);
-            } else {
-              float4 *dst = reinterpret_cast<float4 *>(part + 32 * c + 8 * j);
-              dst[0] = make_float4(e[0], e[1], e[2], e[3]);
-              dst[1] = make_float4(e[4], e[5], e[6], e[7]);
-            }
+            for (int k = 0; k < 8; ++k) h[k] = from_float<OutT>(e[k] * inv);
+            *reinterpret_cast<uint4 *>(s_q + chunk_at(r, 4 * c + j)) =
+                *reinterpret_cast<const uint4 *>(h);
+          } else {
+            float4 *dst = reinterpret_cast<float4 *>(part) + (8 * c + 2 * j) * kRows + tile * kTile + r;
+            dst[0] = make_float4(e[0], e[1], e[2], e[3]);
+            dst[kRows] = make_float4(e[4], e[5], e[6], e[7]);
           }
         }
-        __syncwarp();
       }
-      if (!whole && mine) {
-        part[kKv4D] = m * kScale2;
-        part[kKv4D + 1] = sum;
+      if (whole) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = 2 * i + (lane >> 4), c = lane & 15;
+          const uint64_t to_row = row_at(j);
+          if ((rows >> j) & 1)
+            *reinterpret_cast<uint4 *>(reinterpret_cast<OutT *>(a.out) + to_row + 8 * c) =
+                *reinterpret_cast<const uint4 *>(s_q + chunk_at(r0 + j, c));
+        }
+        __syncwarp();
+      } else {
+        part[kRows * kKv4D + tile * kTile + r] = m * kScale2;
+        part[kRows * (kKv4D + 1) + tile * kTile + r] = sum;
       }
     }
   } else if (warp < kSoftWarps + kDqWarps) {
@@ -616,9 +674,10 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(Kv4AttnArgs a) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int c = c0; c <= c1; ++c) {
-      const float *p = a.parts + (((size_t)c * 2 + (c == c0 ? 1 : 0)) * kRows + (row - rt * kRows)) * kPartRow;
-      const float4 o = *reinterpret_cast<const float4 *>(p + 4 * lane);
-      const float m = p[kKv4D], l = p[kKv4D + 1];
+      const float *p = a.parts + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kPartFloats;
+      const int r = row - rt * kRows;
+      const float4 o = reinterpret_cast<const float4 *>(p)[lane * kRows + r];
+      const float m = p[kRows * kKv4D + r], l = p[kRows * (kKv4D + 1) + r];
       const float up = fmaxf(top, m);
       const float fo = top == up ? 1.f : ex2(top - up), f = m == up ? 1.f : ex2(m - up);
       v.x = v.x * fo + f * o.x;
@@ -655,7 +714,7 @@ int many(mlm_ctx *ctx, const Kv4AttnArgs &a) {
 }  // namespace
 
 size_t kv4_many_parts_bytes(int sm_count) {
-  return sizeof(float) * 2 * sm_count * kRows * kPartRow;
+  return sizeof(float) * 2 * sm_count * kPartFloats;
 }
 
 int kv4_attn_many_init(mlm_ctx *ctx) {
