@@ -5,9 +5,9 @@
 // pairs, token first, so a group's heads share every key tile.  A CTA takes 256
 // rows (two tiles of 128) against tiles of 128 keys, both products on tcgen05
 // with fp32 accumulators in TMEM (M = N = 128):
-//   - 4 warps turn a key tile's cache rows into fp16 K and V in shared memory
+//   - 4 warps each turn a key tile's cache rows into fp16 K and V in shared memory
 //     (a thread per key; one rounding of m + d c, as the read-back gives it), two
-//     buffers;
+//     buffers of each, handed back as soon as their last product is done;
 //   - one thread issues S = Q K^T and O += P V, the two row tiles in turn, so
 //     that one tile's softmax runs while the other's products do;
 //   - 4 warps per row tile do the softmax, a thread per row: S from TMEM, the
@@ -42,13 +42,21 @@ namespace {
 
 constexpr int kTile = 128;          // rows of a row tile, keys of a key tile
 constexpr int kRows = 2 * kTile;    // rows of an item
-constexpr int kSoftWarps = 8, kDqWarps = 4;
-constexpr int kThreads = 32 * (kSoftWarps + kDqWarps + 1);
+constexpr int kSoftWarps = 8, kDqWarps = 8;  // the latter: 4 for K, 4 for V
+constexpr int kMmaWarp = kSoftWarps + kDqWarps;
+constexpr int kThreads = 32 * (kMmaWarp + 4);  // whole warpgroups; three warps idle
+// registers per thread: at launch, then per role; the roles' sum stays below the
+// launch's (65536 / kThreads rounded down to a multiple of 8)
+constexpr int kLaunchRegs = 96, kSoftRegs = 136, kDqRegs = 72, kMmaRegs = 64;
+static_assert(32 * kSoftWarps * kSoftRegs + 32 * kDqWarps * kDqRegs + 128 * kMmaRegs <=
+                  kThreads * kLaunchRegs,
+              "the roles' registers");
 constexpr int kSub = kTile * 128;           // 64 dimensions of a tile: 128 rows x 128 bytes
 constexpr int kOperand = 2 * kSub;          // 32 KB: Q, K or V of a tile
 constexpr int kOffKv = 2 * kOperand;        // after Q of two tiles
 constexpr int kOffBar = kOffKv + 4 * kOperand;
-enum { kQfull = 0, kSfull = 1, kPfull = 3, kOfull = 5, kKvFull = 7, kKvEmpty = 9, kDrain = 11, kBars = 12 };
+enum { kQfull = 0, kSfull = 1, kPfull = 3, kOfull = 5, kKfull = 7, kVfull = 9, kKempty = 11, kVempty = 13,
+       kDrain = 15, kBars = 16 };
 constexpr int kOffTmem = kOffBar + 8 * kBars;
 constexpr int kOffLine = kOffTmem + 16;     // [batch + 1] 64-bit offsets
 constexpr size_t smem_bytes(int batch) { return kOffLine + 8 * (size_t)(batch + 1); }
@@ -66,31 +74,36 @@ constexpr uint32_t kIdescO = kIdescS | (1u << 16);
 // of 1024 bytes, 16-byte chunk c of row r at c ^ (r & 7); version 1, layout type
 // 2.  K-major: atoms 1024 bytes apart along the rows.  N-major: 8-key groups
 // 1024 bytes apart, 64-dimension halves kSub bytes apart.
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ uint64_t desc_n_major(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kSub >> 4) << 16) |
-         ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// The high words are alike; a low word is the address in 16-byte units (shared
+// memory's addresses fit the field) and the other stride, so a step along K is one
+// addition.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k_major(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_n_major(uint32_t addr) {
+  return (addr >> 4) | ((uint32_t)(kSub >> 4) << 16);
 }
 // byte offset of 16-byte chunk c (0 .. 15) of row r in an operand
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return (uint32_t)((c >> 3) * kSub + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t acc) {
+// One thread issues all products, and each takes the tensor cores 64 cycles: the
+// operands' descriptors are low words that change by constants.
+template <bool ACC>
+__device__ __forceinline__ void mma_smem(uint32_t d, uint32_t a, uint32_t b) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(kIdescS), "r"(acc)
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %5, 0;\n"
+      " mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "n"(kDescHi), "n"(kIdescS), "n"(ACC ? 1 : 0)
       : "memory");
 }
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t acc) {
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(kIdescO), "r"(acc)
+      "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %5, 0;\n"
+      " mov.b64 db, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "n"(kDescHi), "n"(kIdescO), "r"(acc)
       : "memory");
 }
 __device__ __forceinline__ void commit(uint32_t bar) {
@@ -279,13 +292,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
       mbar_init(bar + 8 * (kSfull + i), 1);
       mbar_init(bar + 8 * (kPfull + i), kTile);
       mbar_init(bar + 8 * (kOfull + i), 1);
-      mbar_init(bar + 8 * (kKvFull + i), kDqWarps);
-      mbar_init(bar + 8 * (kKvEmpty + i), 1);
+      mbar_init(bar + 8 * (kKfull + i), kDqWarps / 2);
+      mbar_init(bar + 8 * (kVfull + i), kDqWarps / 2);
+      mbar_init(bar + 8 * (kKempty + i), 1);
+      mbar_init(bar + 8 * (kVempty + i), 1);
     }
     mbar_init(bar + 8 * kDrain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kSoftWarps + kDqWarps) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      (uint32_t)__cvta_generic_to_shared(tmem_slot)),
                  "r"(kTmemCols));
@@ -337,6 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
   Walk walk(a, s_off, x0, x1);
   bool ok = true;
   if (warp < kSoftWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     // ---- softmax: a thread per row of tile `tile` --------------------------------
     const int tile = warp >> 2, r = threadIdx.x & (kTile - 1);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -521,23 +537,26 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
         part[kRows * (kKv4D + 1) + tile * kTile + r] = sum;
       }
     }
-  } else if (warp < kSoftWarps + kDqWarps) {
+  } else if (warp < kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDqRegs));
     // ---- cache rows to fp16 operands: a thread per key of the tile ----------------
-    const int key = threadIdx.x - 32 * kSoftWarps;
+    const int key = (threadIdx.x - 32 * kSoftWarps) & (kTile - 1);
+    const bool is_v = warp >= kSoftWarps + kDqWarps / 2;
+    const uint8_t *cache = is_v ? a.vc : a.kc;
+    const uint32_t full = bar + 8 * (is_v ? kVfull : kKfull), empty = bar + 8 * (is_v ? kVempty : kKempty);
     uint32_t n_kv = 0;
-    uint4 raw[10];
+    uint4 raw[5], v_scales = {};  // K's threads also look at their key's value scales
     auto load = [&](const Part &p, int kt) {
       const int j = kt * kTile + key;
       if (j < p.len) {
         const size_t at = (((size_t)p.b * a.n_kv + p.h) * a.capacity + j) * kKv4Row;
 #pragma unroll
-        for (int i = 0; i < 5; ++i) {
-          raw[i] = *reinterpret_cast<const uint4 *>(a.kc + at + 16 * i);
-          raw[5 + i] = *reinterpret_cast<const uint4 *>(a.vc + at + 16 * i);
-        }
+        for (int i = 0; i < 5; ++i) raw[i] = *reinterpret_cast<const uint4 *>(cache + at + 16 * i);
+        v_scales = is_v ? raw[4] : *reinterpret_cast<const uint4 *>(a.vc + at + 64);
       } else {  // past the sequence: zeros
 #pragma unroll
-        for (int i = 0; i < 10; ++i) raw[i] = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 5; ++i) raw[i] = make_uint4(0, 0, 0, 0);
+        v_scales = raw[4];
       }
     };
     bool more = walk.next();
@@ -546,87 +565,89 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
     while (more) {
       const uint32_t buf = n_kv & 1;
       if (n_kv >= 2) {
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar + 8 * (kKvEmpty + buf),
-                                                       ((n_kv >> 1) - 1) & 1, a.status));
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait_bounded(empty + 8 * buf, ((n_kv >> 1) - 1) & 1, a.status));
         if (!ok) break;
       }
-      uint4 cur[10];
+      uint4 cur[5];
 #pragma unroll
-      for (int i = 0; i < 10; ++i) cur[i] = raw[i];
+      for (int i = 0; i < 5; ++i) cur[i] = raw[i];
+      if (not_finite(v_scales.x) || not_finite(v_scales.y) || not_finite(v_scales.z) ||
+          not_finite(v_scales.w)) {
+        const uint32_t x = is_v ? 0u : 0x7FFF7FFFu;
+        cur[4] = make_uint4(x, x, x, x);
+      }
       if (++kt == walk.p.kt1) {
         more = walk.next();
         kt = walk.p.kt0;
       }
       if (more) load(walk.p, kt);
-      const bool bad = not_finite(cur[9].x) || not_finite(cur[9].y) || not_finite(cur[9].z) ||
-                       not_finite(cur[9].w);
-      if (bad) {
+      uint8_t *dst = smem + kOffKv + (2 * buf + is_v) * kOperand;
 #pragma unroll
-        for (int i = 5; i < 10; ++i) cur[i] = make_uint4(0, 0, 0, 0);
-        cur[4] = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
-      }
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t dm = u4_get(cur[4], g);
+        const uint32_t dd = __byte_perm(dm, dm, 0x1010), mm = __byte_perm(dm, dm, 0x3232);
+        const __half2 d = *reinterpret_cast<const __half2 *>(&dd),
+                      m = *reinterpret_cast<const __half2 *>(&mm);
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        uint8_t *dst = smem + kOffKv + (2 * buf + kv) * kOperand;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const uint32_t dm = u4_get(cur[5 * kv + 4], g);
-          const uint32_t dd = __byte_perm(dm, dm, 0x1010), mm = __byte_perm(dm, dm, 0x3232);
-          const __half2 d = *reinterpret_cast<const __half2 *>(&dd),
-                        m = *reinterpret_cast<const __half2 *>(&mm);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<uint4 *>(dst + chunk_at(key, 4 * g + i)) =
-                values8(u4_get(cur[5 * kv + g], i), d, m);
-        }
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint4 *>(dst + chunk_at(key, 4 * g + i)) = values8(u4_get(cur[g], i), d, m);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) arrive(bar + 8 * (kKvFull + buf));
+      if (lane == 0) arrive(full + 8 * buf);
       ++n_kv;
     }
-  } else if (lane == 0) {
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+    if (warp == kMmaWarp && lane == 0) {
     // ---- the products -----------------------------------------------------------
     uint32_t n_kv = 0, n_p[2] = {0, 0}, n_item = 0;
+    const uint32_t q0 = desc_k_major(sbase), k0 = desc_k_major(sbase + kOffKv),
+                   v0 = desc_n_major(sbase + kOffKv + kOperand);
     auto scores = [&](int tile, uint32_t buf) {
-      const uint32_t qa = sbase + tile * kOperand, ka = sbase + kOffKv + 2 * buf * kOperand;
+      const uint32_t q = q0 + tile * (kOperand >> 4), kb = k0 + buf * (2 * kOperand >> 4);
+      const uint32_t d = tmem + tile * kTile;
+      mma_smem<false>(d, q, kb);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t o = (k >> 2) * kSub + (k & 3) * 32;
-        mma_smem(tmem + tile * kTile, desc_k_major(qa + o), desc_k_major(ka + o), k > 0);
+      for (int k = 1; k < 8; ++k) {
+        constexpr int kStep = 32 >> 4, kHalf = kSub >> 4;
+        mma_smem<true>(d, q + (k >> 2) * kHalf + (k & 3) * kStep,
+                       kb + (k >> 2) * kHalf + (k & 3) * kStep);
       }
       commit(bar + 8 * (kSfull + tile));
     };
-    auto kv_ready = [&](uint32_t n) {
-      return mbar_wait_bounded(bar + 8 * (kKvFull + (n & 1)), (n >> 1) & 1, a.status);
+    auto ready = [&](int which, uint32_t n) {
+      const bool in_time = mbar_wait_bounded(bar + 8 * (which + (n & 1)), (n >> 1) & 1, a.status);
+      tc_fence_after();
+      return in_time;
     };
     while (ok && walk.next()) {
       const Part p = walk.p;
       const int tiles = p.count * a.group - p.rt * kRows > kTile ? 2 : 1;
-      ok = mbar_wait_bounded(bar + 8 * kQfull, n_item & 1, a.status) && kv_ready(n_kv);
+      ok = mbar_wait_bounded(bar + 8 * kQfull, n_item & 1, a.status) && ready(kKfull, n_kv);
       if (!ok) break;
       ++n_item;
-      tc_fence_after();
       for (int i = 0; i < tiles; ++i) scores(i, n_kv & 1);
+      commit(bar + 8 * (kKempty + (n_kv & 1)));
       for (int kt = p.kt0; ok && kt < p.kt1; ++kt, ++n_kv) {
-        const uint32_t va = sbase + kOffKv + (2 * (n_kv & 1) + 1) * kOperand;
+        const uint32_t vb = v0 + (n_kv & 1) * (2 * kOperand >> 4);
         for (int i = 0; i < tiles; ++i) {
-          ok = mbar_wait_bounded(bar + 8 * (kPfull + i), n_p[i] & 1, a.status);
+          ok = (i > 0 || ready(kVfull, n_kv)) &&
+               mbar_wait_bounded(bar + 8 * (kPfull + i), n_p[i] & 1, a.status);
           if (!ok) break;
           ++n_p[i];
           tc_fence_after();
+          mma_tmem(tmem + (2 + i) * kTile, tmem + i * kTile, vb, kt > p.kt0);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            mma_tmem(tmem + (2 + i) * kTile, tmem + i * kTile + 8 * k, desc_n_major(va + 2048 * k),
-                     kt > p.kt0 || k > 0);
-          if (i == tiles - 1) commit(bar + 8 * (kKvEmpty + (n_kv & 1)));
+          for (int k = 1; k < 8; ++k)
+            mma_tmem(tmem + (2 + i) * kTile, tmem + i * kTile + 8 * k, vb + k * (2048 >> 4), 1);
+          if (i == tiles - 1) commit(bar + 8 * (kVempty + (n_kv & 1)));
           if (kt + 1 < p.kt1) {
-            if (i == 0) {
-              ok = kv_ready(n_kv + 1);
-              if (!ok) break;
-              tc_fence_after();
-            }
+            ok = i > 0 || ready(kKfull, n_kv + 1);
+            if (!ok) break;
             scores(i, (n_kv + 1) & 1);
+            if (i == tiles - 1) commit(bar + 8 * (kKempty + ((n_kv + 1) & 1)));
           } else {
             commit(bar + 8 * (kOfull + i));
           }
@@ -636,63 +657,68 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
     // nothing of this CTA is in flight when its TMEM and shared memory go
     commit(bar + 8 * kDrain);
     mbar_wait_bounded(bar + 8 * kDrain, 0, a.status);
+    }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kSoftWarps + kDqWarps) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
   }
 }
 
-// Joins the parts of items that several CTAs shared: a warp per output row, four
-// dimensions per lane, the parts in order.
+// Joins the parts of items that several CTAs shared, in order: a CTA per 8 rows of
+// a KV head, a thread per row and four dimensions (8 rows of four dimensions are a
+// line of a part).
+constexpr int kJoinRows = 8;
 template <class OutT>
-__global__ void __launch_bounds__(256) kv4_attn_join_kernel(Kv4AttnArgs a) {
+__global__ void __launch_bounds__(32 * kJoinRows) kv4_attn_join_kernel(Kv4AttnArgs a, int groups) {
   pdl_wait_then_release();
   const int lane = threadIdx.x & 31;
   const long long *plan = reinterpret_cast<const long long *>(a.plan);
-  const long long rows = (long long)a.batch * a.tokens * a.n_heads;
-  const long long quota = plan[0];
-  for (long long i = (long long)blockIdx.x * 8 + threadIdx.x / 32; i < rows; i += gridDim.x * 8ll) {
-    const int head = (int)(i % a.n_heads), t = (int)(i / a.n_heads % a.tokens);
-    const int b = (int)(i / a.n_heads / a.tokens);
-    int len, count;
-    seq_shape(a, b, len, count);
-    if (t >= count) continue;
-    const int h = head / a.group, row = t * a.group + head - h * a.group, rt = row / kRows;
-    const int nkt = key_tiles(len, count, a.group, rt);
-    if (nkt == 0) continue;
-    long long before = 0;
-    for (int k = lane; k < rt; k += 32) before += key_tiles(len, count, a.group, k);
+  const int rg = blockIdx.x % groups, h = blockIdx.x / groups % a.n_kv;
+  const int b = blockIdx.x / groups / a.n_kv;
+  const long long quota = plan[0], first = plan[1 + b];
+  int len, count;
+  seq_shape(a, b, len, count);
+  const int row = rg * kJoinRows + (threadIdx.x & 7), c4 = threadIdx.x >> 3;
+  if (rg * kJoinRows >= count * a.group) return;
+  const int rt = rg * kJoinRows / kRows;
+  const int nkt = key_tiles(len, count, a.group, rt);
+  if (nkt == 0) return;
+  long long before = 0;
+  for (int k = lane; k < rt; k += 32) before += key_tiles(len, count, a.group, k);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-    const long long x = plan[1 + b] + before * a.n_kv + (long long)h * nkt;
-    const int c0 = (int)(x / quota), c1 = (int)((x + nkt - 1) / quota);
-    if (c0 == c1) continue;
-    float top = -INFINITY, sum = 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const float *p = a.parts + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kPartFloats;
-      const int r = row - rt * kRows;
-      const float4 o = reinterpret_cast<const float4 *>(p)[lane * kRows + r];
-      const float m = p[kRows * kKv4D + r], l = p[kRows * (kKv4D + 1) + r];
-      const float up = fmaxf(top, m);
-      const float fo = top == up ? 1.f : ex2(top - up), f = m == up ? 1.f : ex2(m - up);
-      v.x = v.x * fo + f * o.x;
-      v.y = v.y * fo + f * o.y;
-      v.z = v.z * fo + f * o.z;
-      v.w = v.w * fo + f * o.w;
-      sum = sum * fo + f * l;
-      top = up;
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    OutT e[4] = {from_float<OutT>(v.x * inv), from_float<OutT>(v.y * inv),
-                 from_float<OutT>(v.z * inv), from_float<OutT>(v.w * inv)};
-    *reinterpret_cast<uint2 *>(reinterpret_cast<OutT *>(a.out) + (size_t)i * kKv4D + 4 * lane) =
-        *reinterpret_cast<const uint2 *>(e);
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  const long long x = first + before * a.n_kv + (long long)h * nkt;
+  const int c0 = (int)(x / quota), c1 = (int)((x + nkt - 1) / quota);
+  if (c0 == c1) return;
+  const int r = row - rt * kRows;
+  auto part_of = [&](int c) { return a.parts + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kPartFloats; };
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll 8
+  for (int c = c0; c <= c1; ++c) top = fmaxf(top, part_of(c)[kRows * kKv4D + r]);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int c = c0; c <= c1; ++c) {
+    const float *p = part_of(c);
+    const float4 o = reinterpret_cast<const float4 *>(p)[c4 * kRows + r];
+    const float m = p[kRows * kKv4D + r], l = p[kRows * (kKv4D + 1) + r];
+    const float f = m == top ? 1.f : ex2(m - top);
+    v.x = fmaf(f, o.x, v.x);
+    v.y = fmaf(f, o.y, v.y);
+    v.z = fmaf(f, o.z, v.z);
+    v.w = fmaf(f, o.w, v.w);
+    sum = fmaf(f, l, sum);
   }
+  if (row >= count * a.group) return;
+  const int t = row / a.group;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  OutT e[4] = {from_float<OutT>(v.x * inv), from_float<OutT>(v.y * inv),
+               from_float<OutT>(v.z * inv), from_float<OutT>(v.w * inv)};
+  *reinterpret_cast<uint2 *>(reinterpret_cast<OutT *>(a.out) +
+                             (((size_t)b * a.tokens + t) * a.n_heads + h * a.group + row -
+                              t * a.group) * kKv4D + 4 * c4) = *reinterpret_cast<const uint2 *>(e);
 }
 
 template <class OutT>
@@ -702,12 +728,11 @@ int many(mlm_ctx *ctx, const Kv4AttnArgs &a) {
                                              dim3(kThreads), smem_bytes(a.batch), ctx->stream, a),
                                   "mlm_attn_kv4");
   if (st != MLM_OK) return st;
-  const long long rows = (long long)a.batch * a.tokens * a.n_heads;
+  const int groups = (a.tokens * a.group + kJoinRows - 1) / kJoinRows;
   return check_launch_pdl(
       ctx,
-      launch_pdl(kv4_attn_join_kernel<OutT>,
-                 dim3((unsigned)std::min<long long>((rows + 7) / 8, 8ll * ctx->sm_count)), dim3(256),
-                 0, ctx->stream, a),
+      launch_pdl(kv4_attn_join_kernel<OutT>, dim3((unsigned)groups * a.n_kv * a.batch),
+                 dim3(32 * kJoinRows), 0, ctx->stream, a, groups),
       "mlm_attn_kv4 (join)");
 }
 
