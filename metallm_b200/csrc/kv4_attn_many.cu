@@ -667,23 +667,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
   }
 }
 
-// Joins the parts of items that several CTAs shared, in order: a CTA per 8 rows of
-// a KV head, a thread per row and four dimensions (8 rows of four dimensions are a
-// line of a part).
-constexpr int kJoinRows = 8;
+// Joins the parts of items that several CTAs shared, in order: a CTA per 32 rows of
+// a KV head, a thread per four dimensions (8 rows of four dimensions are a line of a
+// part) of four rows, whose loads are in flight together.
+constexpr int kJoinRows = 32;
 template <class OutT>
-__global__ void __launch_bounds__(32 * kJoinRows) kv4_attn_join_kernel(Kv4AttnArgs a, int groups) {
-  pdl_wait_then_release();
+__global__ void __launch_bounds__(256) kv4_attn_join_kernel(Kv4AttnArgs a, int groups) {
   const int lane = threadIdx.x & 31;
-  const long long *plan = reinterpret_cast<const long long *>(a.plan);
   const int rg = blockIdx.x % groups, h = blockIdx.x / groups % a.n_kv;
   const int b = blockIdx.x / groups / a.n_kv;
+  pdl_wait_then_release();
+  const long long *plan = reinterpret_cast<const long long *>(a.plan);
   const long long quota = plan[0], first = plan[1 + b];
   int len, count;
   seq_shape(a, b, len, count);
-  const int row = rg * kJoinRows + (threadIdx.x & 7), c4 = threadIdx.x >> 3;
-  if (rg * kJoinRows >= count * a.group) return;
-  const int rt = rg * kJoinRows / kRows;
+  const int row0 = rg * kJoinRows, rt = row0 / kRows;
+  if (row0 >= count * a.group) return;
   const int nkt = key_tiles(len, count, a.group, rt);
   if (nkt == 0) return;
   long long before = 0;
@@ -693,32 +692,50 @@ __global__ void __launch_bounds__(32 * kJoinRows) kv4_attn_join_kernel(Kv4AttnAr
   const long long x = first + before * a.n_kv + (long long)h * nkt;
   const int c0 = (int)(x / quota), c1 = (int)((x + nkt - 1) / quota);
   if (c0 == c1) return;
-  const int r = row - rt * kRows;
+  const int r = row0 - rt * kRows + (threadIdx.x & 7), c4 = threadIdx.x >> 3;
   auto part_of = [&](int c) { return a.parts + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kPartFloats; };
-  float top = -INFINITY, sum = 0.f;
-#pragma unroll 8
-  for (int c = c0; c <= c1; ++c) top = fmaxf(top, part_of(c)[kRows * kKv4D + r]);
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+  float top[4], sum[4] = {};
+  float4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    top[i] = -INFINITY;
+    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll 2
   for (int c = c0; c <= c1; ++c) {
     const float *p = part_of(c);
-    const float4 o = reinterpret_cast<const float4 *>(p)[c4 * kRows + r];
-    const float m = p[kRows * kKv4D + r], l = p[kRows * (kKv4D + 1) + r];
-    const float f = m == top ? 1.f : ex2(m - top);
-    v.x = fmaf(f, o.x, v.x);
-    v.y = fmaf(f, o.y, v.y);
-    v.z = fmaf(f, o.z, v.z);
-    v.w = fmaf(f, o.w, v.w);
-    sum = fmaf(f, l, sum);
+    float4 o[4];
+    float m[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[i] = reinterpret_cast<const float4 *>(p)[c4 * kRows + r + 8 * i];
+      m[i] = p[kRows * kKv4D + r + 8 * i];
+      l[i] = p[kRows * (kKv4D + 1) + r + 8 * i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float up = fmaxf(top[i], m[i]);
+      const float fo = top[i] == up ? 1.f : ex2(top[i] - up), f = m[i] == up ? 1.f : ex2(m[i] - up);
+      v[i].x = fmaf(f, o[i].x, v[i].x * fo);
+      v[i].y = fmaf(f, o[i].y, v[i].y * fo);
+      v[i].z = fmaf(f, o[i].z, v[i].z * fo);
+      v[i].w = fmaf(f, o[i].w, v[i].w * fo);
+      sum[i] = fmaf(f, l[i], sum[i] * fo);
+      top[i] = up;
+    }
   }
-  if (row >= count * a.group) return;
-  const int t = row / a.group;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  OutT e[4] = {from_float<OutT>(v.x * inv), from_float<OutT>(v.y * inv),
-               from_float<OutT>(v.z * inv), from_float<OutT>(v.w * inv)};
-  *reinterpret_cast<uint2 *>(reinterpret_cast<OutT *>(a.out) +
-                             (((size_t)b * a.tokens + t) * a.n_heads + h * a.group + row -
-                              t * a.group) * kKv4D + 4 * c4) = *reinterpret_cast<const uint2 *>(e);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = rt * kRows + r + 8 * i;
+    if (row >= count * a.group) continue;
+    const int t = row / a.group;
+    const float inv = sum[i] == 0.f ? 0.f : 1.f / sum[i];
+    OutT e[4] = {from_float<OutT>(v[i].x * inv), from_float<OutT>(v[i].y * inv),
+                 from_float<OutT>(v[i].z * inv), from_float<OutT>(v[i].w * inv)};
+    *reinterpret_cast<uint2 *>(reinterpret_cast<OutT *>(a.out) +
+                               (((size_t)b * a.tokens + t) * a.n_heads + h * a.group + row -
+                                t * a.group) * kKv4D + 4 * c4) = *reinterpret_cast<const uint2 *>(e);
+  }
 }
 
 template <class OutT>
@@ -732,7 +749,7 @@ int many(mlm_ctx *ctx, const Kv4AttnArgs &a) {
   return check_launch_pdl(
       ctx,
       launch_pdl(kv4_attn_join_kernel<OutT>, dim3((unsigned)groups * a.n_kv * a.batch),
-                 dim3(32 * kJoinRows), 0, ctx->stream, a, groups),
+                 dim3(256), 0, ctx->stream, a, groups),
       "mlm_attn_kv4 (join)");
 }
 
