@@ -244,22 +244,39 @@ class Context:
     def kv4_append(self, cache: Kv4Cache, k, v, type: int, row_stride: int, tokens: int, pos,
                    counts=None) -> None:
         """Quantize K and V rows into the cache from row pos[b] on."""
-        self.call("mlm_kv4_append", cache, k, v, type, row_stride, tokens, pos, counts)
+        st = self.lib.mlm_kv4_append(self.handle, cache, _address(k), _address(v), type, row_stride,
+                                     tokens, _address(pos), _address(counts))
+        if st:
+            self._check(st, "mlm_kv4_append")
 
     def kv4_read_f16(self, cache: Kv4Cache, tokens: int, pos, counts, k_out, v_out) -> None:
         """The fp16 values that cache rows pos[b] .. stand for."""
-        self.call("mlm_kv4_read_f16", cache, tokens, pos, counts, k_out, v_out)
+        st = self.lib.mlm_kv4_read_f16(self.handle, cache, tokens, _address(pos), _address(counts),
+                                       _address(k_out), _address(v_out))
+        if st:
+            self._check(st, "mlm_kv4_read_f16")
 
     def attn_kv4(self, cache: Kv4Cache, q, n_heads: int, tokens: int, lengths, counts, out,
                  out_type: int = TYPE_F16) -> None:
         """Causal grouped-query attention of `tokens` new tokens per sequence."""
-        self.call("mlm_attn_kv4", cache, q, n_heads, tokens, lengths, counts, out, out_type)
+        st = self.lib.mlm_attn_kv4(self.handle, cache, _address(q), n_heads, tokens,
+                                   _address(lengths), _address(counts), _address(out), out_type)
+        if st:
+            self._check(st, "mlm_attn_kv4")
 
     def sample_f32(self, logits, rows: int, n: int, row_stride: int, params, uniform, tokens_out,
                    prob_out=None) -> None:
         """One token per row of logits by temperature, top-k, top-p and min-p."""
-        self.call("mlm_sample_f32", logits, rows, n, row_stride, params, uniform, tokens_out,
-                  prob_out)
+        st = self.lib.mlm_sample_f32(self.handle, _address(logits), rows, n, row_stride,
+                                     _address(params), _address(uniform), _address(tokens_out),
+                                     _address(prob_out))
+        if st:
+            self._check(st, "mlm_sample_f32")
+
+
+def _address(a):
+    """The device address of a DeviceBuffer, or the address (or None) itself."""
+    return a.ptr if type(a) is DeviceBuffer else a
 
 
 class Kv4Buffers(Kv4Cache):
