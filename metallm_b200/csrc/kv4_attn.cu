@@ -107,6 +107,16 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_
       "l"(src), "r"(bytes), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b),
+                            *reinterpret_cast<const __half2 *>(&c));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+
 // an item (the blocks of one KV head of one sequence) and a block of it
 struct Item {
   int b, h, blk, nb;
@@ -131,6 +141,8 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
   int *s_off = reinterpret_cast<int *>(s_head + W * kPiece);  // [batch + 1]
   __shared__ __align__(8) uint64_t s_bar[W][STAGES];
   __shared__ int s_item[2 * W], s_bh[2 * W];  // pieces: the item's first block (-1: none), b and h
+  // per warp, out of the registers: the item at hand and the one being copied
+  __shared__ Item s_cur[W], s_ahead[W];
   __shared__ int s_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = lane >> 2, t4 = lane & 3;
@@ -212,18 +224,27 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
   auto source = [&](const Item &c) {
     return a.kc + (((size_t)c.b * a.n_kv + c.h) * a.capacity + (size_t)c.blk * kBlk) * kRow;
   };
-  Item cur = {}, ahead = {};
   const uint8_t *src = nullptr;  // the next block to copy
   const long long k_to_v = a.vc - a.kc;
-  int to_copy = w1 - w0;
+  int to_copy = w1 - w0, rows_ahead = 0;  // blocks of this stretch, rows of the item, to come
+  int blk = 0;                            // of the item at hand
+  auto keep = [&](Item &slot, const Item &c) {
+    __syncwarp();
+    if (lane == 0) slot = c;
+    __syncwarp();
+  };
   if (to_copy > 0) {
-    cur = ahead = at(w0);
-    src = source(ahead);
+    const Item c = at(w0);
+    keep(s_cur[warp], c);
+    keep(s_ahead[warp], c);
+    src = source(c);
+    rows_ahead = c.len - c.blk * kBlk;
+    blk = c.blk;
   }
   // copy the next block into a stage and move on
   auto copy = [&](int stage) {
     if (lane == 0) {
-      const uint32_t bytes = (uint32_t)min(kBlk, ahead.len - ahead.blk * kBlk) * kRow;
+      const uint32_t bytes = (uint32_t)min(kBlk, rows_ahead) * kRow;
       const uint32_t bar = bar0 + 8 * stage, dst = ring + stage * kStage;
       mbar_expect_tx(bar, 2 * bytes);
       bulk_copy(dst, src, bytes, bar);
@@ -231,33 +252,20 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
     }
     --to_copy;
     src += kHalfStage;
-    if (++ahead.blk == ahead.nb && to_copy > 0) {
-      next_item(ahead);
-      src = source(ahead);
+    rows_ahead -= kBlk;
+    if (rows_ahead <= 0 && to_copy > 0) {
+      Item c = s_ahead[warp];
+      next_item(c);
+      keep(s_ahead[warp], c);
+      src = source(c);
+      rows_ahead = c.len;
     }
   };
 #pragma unroll
   for (int i = 0; i < STAGES; ++i)
     if (to_copy > 0) copy(i);
 
-  // B operands of the V product: the weights as fp16, hi and lo where both are
-  // wanted; with shared columns a lane's b is one or the other
-  const float part = kSplit && r >= 4 ? 1.f : 0.f;
-  auto split = [&](float v0, float v1, float v2, float v3, uint32_t &b0, uint32_t &b1, uint32_t &l0,
-                   uint32_t &l1) {
-    b0 = pack_f16(v0, v1);
-    b1 = pack_f16(v2, v3);
-    l0 = l1 = 0;
-    if (!LO) return;
-    const float2 h0 = unpack_f16(b0), h1 = unpack_f16(b1);
-    if (DUP) {
-      b0 = pack_f16(fmaf(-part, h0.x, v0), fmaf(-part, h0.y, v1));
-      b1 = pack_f16(fmaf(-part, h1.x, v2), fmaf(-part, h1.y, v3));
-    } else {
-      l0 = pack_f16(v0 - h0.x, v1 - h0.y);
-      l1 = pack_f16(v2 - h1.x, v3 - h1.y);
-    }
-  };
+  const bool lo_lane = kSplit && r >= 4;  // with shared columns: this lane's part
 
   // queries: the B operand of K's products, per group of 32 dimensions
   uint32_t qb[NT][4][4];
@@ -266,18 +274,17 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
   uint32_t qm[NT][2];          // the B operand of K's minima: (0, group sum) per group, hi and lo
   float o[NT][4][2][4], mx[NT], l[NT];
   float om[NT][4];             // sum of p m: rows 2 g + 1 of the product with V's scales
-  float omf[NT][4];            // the same of masked blocks, group g, this lane's rows
-  float slack[NT];             // a score's lead over the maximum that is let pass
   bool ok = true;
   int stage = 0;
   uint32_t phase = 0;
 
   for (int x = w0; x < w1;) {
-    const int first_blk = cur.blk;
-    const int end_blk = min(cur.nb, cur.blk + w1 - x);  // this stretch's part of the item
+    const int first_blk = blk;
+    const int end_blk = min(s_cur[warp].nb, blk + w1 - x);  // this stretch's part of the item
     x += end_blk - first_blk;
     int mask_from;  // the first block with a row that some token does not see
     {
+      const Item cur = s_cur[warp];
       const int len = cur.len, count = cur.count;
       mask_from = max(0, len - count + 1) / kBlk;
 #pragma unroll
@@ -306,7 +313,6 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
         const int e = big > 0.f ? 13 - ((int)((__float_as_uint(big) >> 23) & 0xFF) - 127) : 0;
         const float up = __uint_as_float((uint32_t)(e + 127) << 23);
         cs[nt] = kInvSqrtD * kLog2e * __uint_as_float((uint32_t)(24 - e + 127) << 23);
-        slack[nt] = 8.f / cs[nt];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           float sum = 0.f;
@@ -327,7 +333,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
             qm[nt][0] = pack_f16(0.f, hi);
             qm[nt][1] = pack_f16(0.f, sum - hi);
           }
-          om[nt][g] = omf[nt][g] = 0.f;
+          om[nt][g] = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[nt][g][0][i] = o[nt][g][1][i] = 0.f;
         }
@@ -392,15 +398,31 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
             sT[nt][kt][half][1] = __uint_as_float(__byte_perm(lo, hi, 0x7632));
           }
       }
-      const int row0 = cur.blk * kBlk + 2 * t4;  // this lane's first row of the block
+      // Rows that a column does not see get no weight.  A value row with NaN scales
+      // (0 x NaN is not 0) or past the sequence goes in with zero scales; the NaN shows
+      // in the weight of the columns that see it.
+      uint32_t good = 0xFFu;
       if (MASK) {
+        const int row0 = blk * kBlk + 2 * t4, len = s_cur[warp].len;
+        good = 0;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int i = 0; i < 8; ++i) {
+          const int at = (i >> 2) * 16 + ((i >> 1) & 1) * 8 + (i & 1);
+          const uint4 dm = lds16(sv + (2 * t4 + at) * kRow + 64);
+          const bool bad = not_finite(dm.x) || not_finite(dm.y) || not_finite(dm.z) || not_finite(dm.w);
+          if (row0 + at < len && !bad) good |= 1u << i;
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (row0 + (i >> 2) * 16 + ((i >> 1) & 1) * 8 + (i & 1) >= seen[nt])
-              sT[nt][i >> 2][(i >> 1) & 1][i & 1] = -INFINITY;
+          for (int nt = 0; nt < NT; ++nt) {
+            float &v = sT[nt][i >> 2][(i >> 1) & 1][i & 1];
+            if (bad) v = NAN;
+            if (row0 + at >= seen[nt]) v = -INFINITY;
+          }
+        }
       }
+      auto good_pair = [&](int kt, int j) -> uint32_t {
+        const uint32_t bits = good >> (4 * kt + 2 * j);
+        return ((bits & 1) ? 0xFFFFu : 0u) | ((bits & 2) ? 0xFFFF0000u : 0u);
+      };
       // Running maximum and sum.  The maximum follows only when a score leads it
       // by more than 2^8: the weights are 2^(s - max - 6), so at most 4, and p d stays
       // an fp16 value for every d below 2^14; the factor is l's too.
@@ -409,7 +431,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, sT[nt][i >> 2][(i >> 1) & 1][i & 1]);
-        if (__any_sync(0xffffffffu, top > mx[nt] + slack[nt])) {
+        if (__any_sync(0xffffffffu, (top - mx[nt]) * cs[nt] > 8.f)) {
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           top = fmaxf(top, mx[nt]);
@@ -419,7 +441,6 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
                       f1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            omf[nt][g] *= f;
             om[nt][g] *= (g & 1) ? f1 : f0;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -449,41 +470,66 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           dm[i] = lds16(sv + (kt * 16 + (i >> 1) * 8 + 2 * t4 + (i & 1)) * kRow + 64);
-        if (!MASK) {
-          // sum_j p_j m_jg (and p_j d_jg, unused): the transposed scale words
-          uint32_t mt[2];
-          ldsm2_t(sv + (kt * 16 + (lane & 15)) * kRow + 64, mt);
+        // the weights of the lane's four rows as fp16 hi (and lo) pairs
+        uint32_t ph[NT][2], pl[NT][2], pn[NT][2];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float(&p)[2][2] = sT[nt][kt];
-            uint32_t b0, b1, l0, l1;
-            split(p[0][0], p[0][1], p[1][0], p[1][1], b0, b1, l0, l1);
-            mma_f16_16816(om[nt], mt[0], 0u, mt[1], 0u, b0, b1);
-            if (LO && !DUP) mma_f16_16816(om[nt], mt[0], 0u, mt[1], 0u, l0, l1);
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float(&p)[2] = sT[nt][kt][j];
+            ph[nt][j] = pack_f16(p[0], p[1]);
+            pl[nt][j] = pn[nt][j] = 0;
+            if (LO) {
+              const float2 h = unpack_f16(ph[nt][j]);
+              pl[nt][j] = pack_f16(p[0] - h.x, p[1] - h.y);
+              if (DUP) {
+                pl[nt][j] = lo_lane ? pl[nt][j] : 0u;
+                pn[nt][j] = lo_lane ? ph[nt][j] ^ 0x80008000u : 0u;
+              }
+            }
           }
+        // sum_j p_j m_jg (and p_j d_jg, unused): the transposed scale words
+        uint32_t mt[2];
+        ldsm2_t(sv + (kt * 16 + (lane & 15)) * kRow + 64, mt);
+        if (MASK) {
+          mt[0] &= good_pair(kt, 0);
+          mt[1] &= good_pair(kt, 1);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint32_t b0 = kSplit && lo_lane ? pl[nt][0] : ph[nt][0],
+                         b1 = kSplit && lo_lane ? pl[nt][1] : ph[nt][1];
+          mma_f16_16816(om[nt], mt[0], 0u, mt[1], 0u, b0, b1);
+          if (LO && !DUP) mma_f16_16816(om[nt], mt[0], 0u, mt[1], 0u, pl[nt][0], pl[nt][1]);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const uint32_t wa = w[g >> 1][(g & 1) * 2], wb = w[g >> 1][(g & 1) * 2 + 1];
           const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
+          // d of rows 2 t4, + 1 and of rows 2 t4 + 8, + 9
+          uint32_t dd[2] = {__byte_perm(u4_get(dm[0], g), u4_get(dm[1], g), 0x5410),
+                            __byte_perm(u4_get(dm[2], g), u4_get(dm[3], g), 0x5410)};
+          if (MASK) {
+            dd[0] &= good_pair(kt, 0);
+            dd[1] &= good_pair(kt, 1);
+          }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float v[4];
+            uint32_t bh[2], bl[2] = {0, 0};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float p = sT[nt][kt][i >> 1][i & 1];
-              if (MASK) {
-                // a row this column does not see adds nothing, whatever its scales hold
-                const float2 f = unpack_f16(u4_get(dm[i], g));
-                const bool sees = row0 + kt * 16 + (i >> 1) * 8 + (i & 1) < seen[nt];
-                v[i] = sees ? p * f.x : 0.f;
-                omf[nt][g] += sees ? p * f.y : 0.f;
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t d = dd[j];
+              // p d = hi + lo: hi the rounded product, lo its exact rest and p_lo d
+              if (!LO) {
+                bh[j] = hmul2(ph[nt][j], d);
+              } else if (DUP) {  // hi in lanes with pn = pl = 0, lo in the others
+                bh[j] = hfma2(pl[nt][j], d, hfma2(ph[nt][j], d, hmul2(pn[nt][j], d)));
               } else {
-                v[i] = p * low_f16(u4_get(dm[i], g));
+                bh[j] = hmul2(ph[nt][j], d);
+                bl[j] = hfma2(pl[nt][j], d, hfma2(ph[nt][j], d, bh[j] ^ 0x80008000u));
               }
             }
-            uint32_t b0, b1, l0, l1;
-            split(v[0], v[1], v[2], v[3], b0, b1, l0, l1);
+            const uint32_t b0 = bh[0], b1 = bh[1], l0 = bl[0], l1 = bl[1];
             mma_f16_16816(o[nt][g][0], wa & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x000F000Fu,
                           wb & 0x00F000F0u, b0, b1);
             mma_f16_16816(o[nt][g][1], wa8 & 0x000F000Fu, wa8 & 0x00F000F0u, wb8 & 0x000F000Fu,
@@ -498,10 +544,10 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
         }
       }
     };
-    for (; cur.blk < end_blk; ++cur.blk) {
+    for (; blk < end_blk; ++blk) {
       // after a wait that ran out (status is set) the rest is only walked through
       if (ok) ok = mbar_wait_bounded(bar0 + 8 * stage, phase, a.status);
-      if (cur.blk >= mask_from)
+      if (blk >= mask_from)
         block(std::true_type());
       else
         block(std::false_type());
@@ -515,8 +561,9 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
 
     // the item or the stretch ends: the item's output, or a piece of it
     {
-      const bool item_ends = cur.blk == cur.nb;
-      const int item = x - cur.blk;  // the item's first block on the line
+      Item cur = s_cur[warp];
+      const bool item_ends = blk == cur.nb;
+      const int item = x - blk;  // the item's first block on the line
       const bool whole = item_ends && first_blk == 0;
       const int slot = 2 * warp + (x == w1 ? 1 : 0);
       float *piece = x == w1 ? reinterpret_cast<float *>(smem + warp * STAGES * kStage)
@@ -530,17 +577,12 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
         const float i0 = __shfl_sync(0xffffffffu, inv, 8 * t4), i1 = __shfl_sync(0xffffffffu, inv, 8 * t4 + 4);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          float m = omf[nt][g];
-          m += __shfl_xor_sync(0xffffffffu, m, 1);
-          m += __shfl_xor_sync(0xffffffffu, m, 2);
           float m0 = __shfl_sync(0xffffffffu, om[nt][0], 4 * (2 * g + 1) + t4),
                 m1 = __shfl_sync(0xffffffffu, om[nt][1], 4 * (2 * g + 1) + t4);
           if (kSplit) {
             m0 += __shfl_xor_sync(0xffffffffu, m0, 2);
             m1 += __shfl_xor_sync(0xffffffffu, m1, 2);
           }
-          m0 += __shfl_sync(0xffffffffu, m, 8 * t4);
-          m1 += __shfl_sync(0xffffffffu, m, 8 * t4 + 4);
           float v[2][4];  // columns 2 t4 and 2 t4 + 1, dimensions 32 g + 4 r ..
 #pragma unroll
           for (int i = 0; i < 2; ++i)
@@ -583,7 +625,11 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
         s_item[slot] = item;
         s_bh[slot] = cur.b * a.n_kv + cur.h;
       }
-      if (item_ends && x < w1) next_item(cur);
+      if (item_ends && x < w1) {
+        next_item(cur);
+        keep(s_cur[warp], cur);
+        blk = 0;
+      }
     }
   }
   if (!ok) {  // let this warp's last copies land before its shared memory goes

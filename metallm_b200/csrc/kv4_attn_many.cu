@@ -274,10 +274,6 @@ __device__ __forceinline__ uint4 values8(uint32_t w, __half2 d, __half2 m) {
   }
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
-__device__ __forceinline__ bool not_finite(uint32_t dm) {
-  return (dm & 0x7C00u) == 0x7C00u || (dm & 0x7C000000u) == 0x7C000000u;
-}
-
 template <class OutT>
 __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];

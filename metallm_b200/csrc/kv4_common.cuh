@@ -51,8 +51,16 @@ __device__ __forceinline__ float2 unpack_f16(uint32_t v) {
 __device__ __forceinline__ float low_f16(uint32_t v) {
   return __half2float(__ushort_as_half((unsigned short)v));
 }
+__device__ __forceinline__ float high_f16(uint32_t v) {
+  return __half2float(__ushort_as_half((unsigned short)(v >> 16)));
+}
 __device__ __forceinline__ uint32_t u4_get(const uint4 &v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+// whether a (d, m) pair holds an infinity or NaN
+__device__ __forceinline__ bool not_finite(uint32_t dm) {
+  return (dm & 0x7C00u) == 0x7C00u || (dm & 0x7C000000u) == 0x7C000000u;
 }
 
 // kv4_attn.cu: up to 16 (token, head) rows per KV head; kv4_attn_many.cu: more
