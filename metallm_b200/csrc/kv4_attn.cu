@@ -42,14 +42,14 @@ constexpr int kD = kKv4D;
 // balanced.  A warp streams its blocks through a ring of its own (two 2560-byte
 // bulk copies per block, contiguous in the cache) and keeps a running maximum
 // and sum per column.  Stretches of one head are joined in order: a warp's
-// pieces in shared memory, a CTA's through the context's scratch by the last
-// CTA of the head to arrive, so sums do not depend on timing.
+// pieces by their CTA, the CTAs' through the context's scratch by the last CTA of the
+// head to arrive, so sums do not depend on timing.
 // ---------------------------------------------------------------------------
 
 constexpr int kBlk = 32;                     // cache rows per block
 constexpr int kHalfStage = kBlk * kRow;      // K or V of a block
 constexpr int kStage = 2 * kHalfStage;
-constexpr int kPieceRow = kD + 2;            // a column of a piece: o[128], m, l
+constexpr int kPieceRow = kD + 4;            // a column of a piece: o[128], m, l, padding
 constexpr int kMaxCols = 16;
 
 // a product from zero accumulators
@@ -99,12 +99,14 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
+// (the cache is read once per step: evict-first, so that it does not push the kernel's
+// code and the partial sums out of L2)
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_t bytes,
-                                          uint32_t bar) {
+                                          uint32_t bar, uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          dst),
-      "l"(src), "r"(bytes), "r"(bar)
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint "
+      "[%0], [%1], %2, [%3], %4;" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar), "l"(policy)
       : "memory");
 }
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
@@ -123,6 +125,71 @@ struct Item {
   int len, count;  // of sequence b
 };
 
+// Joins the parts of an item that CTAs c0 .. c1 share, in order: a warp per column and
+// 32 V dimensions, whose parts' loads are in flight together.
+template <int V, class OutT>
+__device__ __forceinline__ void join_parts(const Kv4AttnArgs &a, const Item &of, int c0, int c1,
+                                           int warp, int warps) {
+  static_assert(V == 2 || V == 4, "one load per part");
+  constexpr int kTasks = 4 / V;  // per column
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int t = warp; t < kTasks * of.count * a.group; t += warps) {
+    const int col = t / kTasks, d = (t % kTasks) * 32 * V + V * lane;
+    auto part_of = [&](int c) {
+      return a.parts + (((size_t)c * 2 + (c == c0 ? 1 : 0)) * kMaxCols + col) * kPieceRow;
+    };
+    float top = -INFINITY, sum = 0.f, v[V] = {};
+    // 32 parts at a time, their statistics one per lane; a new maximum rescales
+#pragma unroll 1
+    for (int cb = c0; cb <= c1; cb += 32) {
+      const int n = min(32, c1 - cb + 1);
+      const bool in = lane < n;
+      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(cb + (in ? lane : 0)) + kD));
+      const float m = in ? ml.x : -INFINITY;
+      const float up = fmaxf(top, warp_max(m));
+      const float old = top == up ? 1.f : ex2(top - up), f = m == up ? 1.f : ex2(m - up);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] *= old;
+      sum = sum * old + (in ? f * ml.y : 0.f);
+      top = up;
+#pragma unroll 1
+      for (int k0 = 0; k0 < n; k0 += 8) {
+        float w[8][V];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float *p = part_of(min(cb + k0 + k, c1)) + d;
+          if (V == 4) {
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(p));
+            w[k][0] = x.x, w[k][1] = x.y, w[k][V - 2] = x.z, w[k][V - 1] = x.w;
+          } else {
+            const float2 x = __ldcg(reinterpret_cast<const float2 *>(p));
+            w[k][0] = x.x, w[k][1] = x.y;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float fk = __shfl_sync(0xffffffffu, f, (k0 + k) & 31);
+          if (k0 + k < n)
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = fmaf(fk, w[k][i], v[i]);
+        }
+      }
+    }
+    sum = warp_sum(sum);
+    const int tok = a.tokens == 1 ? 0 : col / a.group;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    OutT *dst = reinterpret_cast<OutT *>(a.out) +
+                (((size_t)of.b * a.tokens + tok) * a.n_heads + of.h * a.group + (col - tok * a.group)) * kD + d;
+    OutT e[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = from_float<OutT>(v[i] * inv);
+#pragma unroll
+    for (int i = 0; i < V; i += 2)
+      *reinterpret_cast<uint32_t *>(dst + i) = *reinterpret_cast<const uint32_t *>(e + i);
+  }
+}
+
 template <int NT, bool DUP, int W, int STAGES, class OutT>
 __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) {
   static_assert(2 * W <= 32, "a lane per piece");
@@ -136,14 +203,14 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
   constexpr bool kSplit = DUP && LO;  // columns 4 .. 7 hold the lo parts
   static_assert(kPiece * 4 <= STAGES * kStage, "a warp's last piece lies in its ring");
   extern __shared__ __align__(128) uint8_t smem[];
-  // rings, the warps' head pieces, the line's offsets per sequence
-  float *s_head = reinterpret_cast<float *>(smem + W * STAGES * kStage);
-  int *s_off = reinterpret_cast<int *>(s_head + W * kPiece);  // [batch + 1]
+  // rings, the line's offsets per sequence
+  int *s_off = reinterpret_cast<int *>(smem + W * STAGES * kStage);  // [batch + 1]
   __shared__ __align__(8) uint64_t s_bar[W][STAGES];
-  __shared__ int s_item[2 * W], s_bh[2 * W];  // pieces: the item's first block (-1: none), b and h
+  __shared__ int s_item[2 * W];  // pieces: the item's first block (-1: none)
+  __shared__ Item s_of[2 * W];   // and the item
+  __shared__ bool s_last[2];
   // per warp, out of the registers: the item at hand and the one being copied
   __shared__ Item s_cur[W], s_ahead[W];
-  __shared__ int s_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = lane >> 2, t4 = lane & 3;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * kStage;
@@ -247,8 +314,9 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
       const uint32_t bytes = (uint32_t)min(kBlk, rows_ahead) * kRow;
       const uint32_t bar = bar0 + 8 * stage, dst = ring + stage * kStage;
       mbar_expect_tx(bar, 2 * bytes);
-      bulk_copy(dst, src, bytes, bar);
-      bulk_copy(dst + kHalfStage, src + k_to_v, bytes, bar);
+      const uint64_t policy = evict_first_policy();
+      bulk_copy(dst, src, bytes, bar, policy);
+      bulk_copy(dst + kHalfStage, src + k_to_v, bytes, bar, policy);
     }
     --to_copy;
     src += kHalfStage;
@@ -261,9 +329,23 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
       rows_ahead = c.len;
     }
   };
+  // the first item's queries into L1, ahead of the copies that would keep them waiting:
+  // two lines per column
+  if (to_copy > 0) {
+    const Item c = s_cur[warp];
+    const int col = lane >> 1, tok = a.tokens == 1 ? 0 : col / a.group;
+    if (col < c.count * a.group)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(
+          a.q + (((size_t)c.b * a.tokens + tok) * a.n_heads + c.h * a.group + (col - tok * a.group)) * kD +
+          64 * (lane & 1)));
+  }
 #pragma unroll
   for (int i = 0; i < STAGES; ++i)
     if (to_copy > 0) copy(i);
+
+  // Pieces that end within a warp's stretch wait in the scratch (the ring is in use);
+  // the stretch's last one lies in the ring
+  float *heads = a.parts + (size_t)2 * gridDim.x * kMaxCols * kPieceRow + (size_t)blockIdx.x * W * kPiece;
 
   const bool lo_lane = kSplit && r >= 4;  // with shared columns: this lane's part
 
@@ -291,7 +373,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
       for (int nt = 0; nt < NT; ++nt) {
         const int col = DUP ? (r & 3) : nt * 8 + r;
         const bool live = col < count * a.group;
-        const int tok = live ? col / a.group : 0;
+        const int tok = live && a.tokens > 1 ? col / a.group : 0;
         seen[nt] = live ? max(0, len - count + tok + 1) : 0;
         const __half *qr = a.q + (((size_t)cur.b * a.tokens + tok) * a.n_heads +
                                   cur.h * a.group + (col - tok * a.group)) * kD + 8 * t4;
@@ -567,7 +649,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
       const bool whole = item_ends && first_blk == 0;
       const int slot = 2 * warp + (x == w1 ? 1 : 0);
       float *piece = x == w1 ? reinterpret_cast<float *>(smem + warp * STAGES * kStage)
-                             : s_head + warp * kPiece;
+                             : heads + warp * kPiece;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int count = cur.count;
@@ -623,7 +705,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
       }
       if (!whole && lane == 0) {
         s_item[slot] = item;
-        s_bh[slot] = cur.b * a.n_kv + cur.h;
+        s_of[slot] = cur;
       }
       if (item_ends && x < w1) {
         next_item(cur);
@@ -640,113 +722,101 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
 
   // Join the pieces.  A slot per lane; an item's pieces are one per warp of a
   // range of warps: in the ring where the warp's stretch ended inside the item, its
-  // head slot where the item ended first.
+  // head piece where the item ended first.  A warp takes a column of an item, a lane
+  // four dimensions and one piece's statistics.
   const int my_item = lane < 2 * W ? s_item[lane] : -1;
-  uint32_t left = __ballot_sync(0xffffffffu, my_item >= 0);
-  while (left) {
+  int task = 0, open0 = -1, open1 = -1;  // slots of items that go beyond this CTA
+  for (uint32_t left = __ballot_sync(0xffffffffu, my_item >= 0); left;) {
     const int s0 = __ffs(left) - 1;
     const int item = __shfl_sync(0xffffffffu, my_item, s0);
     const uint32_t group = __ballot_sync(0xffffffffu, my_item == item) & left;
     left &= ~group;
     const int s1 = 31 - __clz(group);
     const int first_warp = s0 >> 1, n = (s1 >> 1) - first_warp + 1;
-    const int bh = s_bh[s0], b = bh / a.n_kv, h = bh - b * a.n_kv;
-    const int nb = (s_off[b + 1] - s_off[b]) / a.n_kv;
-    const bool complete = item >= cta0 && item + nb <= cta1;
-    int len, count;
-    seq_shape(a, b, len, count);
-    auto piece_of = [&](int i) -> const float * {  // of warp first_warp + i
-      return i == n - 1 && !(s1 & 1)
-                 ? s_head + (first_warp + i) * kPiece
-                 : reinterpret_cast<const float *>(smem + (first_warp + i) * STAGES * kStage);
-    };
-    auto emit = [&](int col, int d, float v) {
-      if (col >= count * a.group) return;
-      const int tok = col / a.group;
-      reinterpret_cast<OutT *>(a.out)[(((size_t)b * a.tokens + tok) * a.n_heads + h * a.group +
-                                       (col - tok * a.group)) * kD + d] = from_float<OutT>(v);
-    };
-    float *mine = a.parts + ((size_t)blockIdx.x * 2 + (item < cta0 ? 0 : 1)) * kMaxCols * kPieceRow;
-    // a warp takes 32 dimensions of a column; lane i holds piece i's statistics
-    for (int i = warp; i < kCols * kD / 32; i += W) {
-      const int col = i / (kD / 32), d = i % (kD / 32) * 32 + lane;
-      const float *pm = piece_of(min(lane, n - 1)) + col * kPieceRow;
-      const float m = lane < n ? pm[kD] : -INFINITY;
+    const bool complete = item >= cta0 && item + s_of[s0].nb <= cta1;
+    for (int col = 0; col < kCols; ++col, ++task) {
+      if (task % W != warp) continue;
+      auto piece_of = [&](int i) -> const float * {  // of warp first_warp + i
+        return (i == n - 1 && !(s1 & 1)
+                    ? heads + (first_warp + i) * kPiece
+                    : reinterpret_cast<const float *>(smem + (first_warp + i) * STAGES * kStage)) +
+               col * kPieceRow;
+      };
+      const float *ps = piece_of(min(lane, n - 1)) + kD;
+      const float m = lane < n ? ps[0] : -INFINITY;
       const float top = warp_max(m);
       const float f = m == top ? 1.f : ex2(m - top);
-      const float sum = warp_sum(lane < n ? f * pm[kD + 1] : 0.f);
-      float v = 0.f;
-#pragma unroll
-      for (int k = 0; k < W; ++k)
-        if (k < n) v = fmaf(__shfl_sync(0xffffffffu, f, k), piece_of(k)[col * kPieceRow + d], v);
+      const float sum = warp_sum(lane < n ? f * ps[1] : 0.f);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+        const float4 w = *reinterpret_cast<const float4 *>(piece_of(k) + 4 * lane);
+        v.x = fmaf(fk, w.x, v.x);
+        v.y = fmaf(fk, w.y, v.y);
+        v.z = fmaf(fk, w.z, v.z);
+        v.w = fmaf(fk, w.w, v.w);
+      }
       if (complete) {
-        emit(col, d, sum == 0.f ? 0.f : v / sum);
-      } else {
-        mine[col * kPieceRow + d] = v;
-        if (d == 0) {
-          mine[col * kPieceRow + kD] = top;
-          mine[col * kPieceRow + kD + 1] = sum;
-        }
+        const Item of = s_of[s0];
+        if (col >= of.count * a.group) continue;
+        const int tok = a.tokens == 1 ? 0 : col / a.group;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        OutT e[4] = {from_float<OutT>(v.x * inv), from_float<OutT>(v.y * inv),
+                     from_float<OutT>(v.z * inv), from_float<OutT>(v.w * inv)};
+        *reinterpret_cast<uint2 *>(reinterpret_cast<OutT *>(a.out) +
+                                   (((size_t)of.b * a.tokens + tok) * a.n_heads + of.h * a.group +
+                                    (col - tok * a.group)) * kD + 4 * lane) =
+            *reinterpret_cast<const uint2 *>(e);
+      } else {  // at most one item that began before this CTA's stretch, one that goes on
+        float *mine = a.parts + (((size_t)blockIdx.x * 2 + (item < cta0 ? 0 : 1)) * kMaxCols + col) *
+                                    kPieceRow;
+        *reinterpret_cast<float4 *>(mine + 4 * lane) = v;
+        if (lane == 0) *reinterpret_cast<float2 *>(mine + kD) = make_float2(top, sum);
       }
     }
-    if (complete) continue;
-    // the last CTA of the item to arrive joins the CTAs' parts, in order
-    const int c0 = item / quota, c1 = (item + nb - 1) / quota;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      s_last = atomicAdd(a.arrivals + c0, 1) == c1 - c0;
-      if (s_last) a.arrivals[c0] = 0;
+    if (!complete) (item < cta0 ? open0 : open1) = s0;
+  }
+  if (open0 < 0 && open1 < 0) return;
+  // the last CTA of such an item to arrive joins the CTAs' parts
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    const int s = threadIdx.x ? open1 : open0;
+    bool last = false;
+    if (s >= 0) {
+      const int item = s_item[s], c0 = item / quota;
+      last = atomicAdd(a.arrivals + c0, 1) == (item + s_of[s].nb - 1) / quota - c0;
+      if (last) a.arrivals[c0] = 0;
     }
-    __syncthreads();
-    if (s_last) {
-      __threadfence();
-      for (int i = warp; i < kCols * kD / 32; i += W) {
-        const int col = i / (kD / 32), d = i % (kD / 32) * 32 + lane;
-        auto part_of = [&](int c) {
-          return a.parts + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kMaxCols * kPieceRow + col * kPieceRow;
-        };
-        float top = -INFINITY, v = 0.f, sum = 0.f;
-        // 32 parts at a time, their statistics one per lane; a new maximum rescales
-        for (int cb = c0; cb <= c1; cb += 32) {
-          const int n1 = min(32, c1 - cb + 1);
-          const bool in = lane < n1;
-          const float *ps = part_of(cb + (in ? lane : 0)) + kD;
-          const float m = in ? __ldcg(ps) : -INFINITY, ls = in ? __ldcg(ps + 1) : 0.f;
-          float w[8];
-          const float up = fmaxf(top, warp_max(m));
-          const float old = top == up ? 1.f : ex2(top - up), f = m == up ? 1.f : ex2(m - up);
-          v *= old;
-          sum = sum * old + (in ? f * ls : 0.f);
-          top = up;
-          for (int k0 = 0; k0 < n1; k0 += 8) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = k0 + k < n1 ? __ldcg(part_of(cb + k0 + k) + d) : 0.f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (k0 + k < n1) v = fmaf(__shfl_sync(0xffffffffu, f, k0 + k), w[k], v);
-          }
-        }
-        sum = warp_sum(sum);
-        emit(col, d, sum == 0.f ? 0.f : v / sum);
-      }
-    }
-    __syncthreads();
+    s_last[threadIdx.x] = last;
+  }
+  __syncthreads();
+  __threadfence();
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    if (!s_last[i]) continue;
+    const int s = i ? open1 : open0, item = s_item[s];
+    const Item of = s_of[s];
+    join_parts<NT == 1 ? 2 : 4, OutT>(a, of, item / quota, (item + of.nb - 1) / quota, warp, W);
   }
 }
 
-// warps and ring stages per column count: the rings hold 140-164 KB in flight
-// per SM beside the warps' head pieces
+// warps (as many on each SM quarter: 14 of them left two quarters idle for a sixth of
+// the time) and ring stages per column count: 160-184 KB in flight per SM
 template <int NT, bool DUP>
 struct FewShape {
-  static constexpr int warps = DUP ? 16 : NT == 1 ? 14 : 12;
-  static constexpr int stages = 2;
+  static constexpr int warps = NT == 1 ? 16 : 8;
+  static constexpr int stages = NT == 1 ? 2 : 4;
   static constexpr int cols = DUP ? 4 : 8 * NT;
   static constexpr size_t smem(int batch) {
-    return (size_t)warps * stages * kStage + (size_t)warps * cols * kPieceRow * 4 +
-           sizeof(int) * (batch + 1);
+    return (size_t)warps * stages * kStage + sizeof(int) * (batch + 1);
   }
 };
+// the CTAs' parts, then the warps' head pieces
+constexpr size_t few_scratch_floats(int sm_count) {
+  return ((size_t)2 * kMaxCols + 16 * kMaxCols) * sm_count * kPieceRow;
+}
 
 template <int NT, bool DUP, class OutT>
 constexpr auto few_kernel() {
@@ -789,7 +859,7 @@ int kv4_attn_init(mlm_ctx *ctx) {
   if (st == MLM_OK) st = few_init<2, false, __nv_bfloat16>(ctx);
   if (st == MLM_OK) st = kv4_attn_many_init(ctx);
   if (st != MLM_OK) return st;
-  const size_t parts = std::max(sizeof(float) * 2 * ctx->sm_count * kMaxCols * kPieceRow,
+  const size_t parts = std::max(sizeof(float) * few_scratch_floats(ctx->sm_count),
                                 kv4_many_parts_bytes(ctx->sm_count));
   if (cudaMalloc(&ctx->kv4_parts, parts) != cudaSuccess ||
       cudaMalloc(&ctx->kv4_arrivals, sizeof(int) * (ctx->sm_count + 1 + kKv4PlanInts)) != cudaSuccess)
