@@ -11,12 +11,14 @@
 //    depend on the run;
 //  - a pass puts every token into one of 2048 bins of (max - x), sums counts or
 //    masses per bin, and a scan finds the bin in which the k-th token, or the
-//    top_p share of the mass, falls.  Where the tokens down to that bin fit a list
-//    (tens, for usual settings) they are gathered and one CTA does the rest on the
-//    list: ranks by counting, masses, both cuts and the draw.  Otherwise the bin's
-//    tokens alone are gathered and give the exact cut, and the draw goes over the
-//    row again; a bin with more tokens than the list holds (flat or constant rows)
-//    is first narrowed by 11-bit digits of the key, which always ends, as keys are
+//    top_p share of the mass, falls.  For a short top-k each CTA does so for its own
+//    slice and sends the slice's first k tokens to the row's first CTA, which sorts
+//    them, takes masses, applies the cuts and draws: one exchange between the CTAs.
+//    Otherwise the CTAs' bins are summed; where the tokens down to the cut's bin fit
+//    the list the same CTA finishes on it, and where they do not the bin's tokens
+//    alone are gathered and give the exact cut, and the draw goes over the row
+//    again.  A bin with more tokens than the list holds (flat or constant rows) is
+//    first narrowed by 11-bit digits of the key, which always ends, as keys are
 //    distinct;
 //  - the draw is by index: masses per warp's stretch of the row, a scan, and the
 //    one stretch that holds the point is walked again by the whole CTA.
@@ -40,26 +42,29 @@ constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kCand = 1024;       // tokens of the list
-constexpr int kMaxCluster = 16;   // of CTAs; above 8 needs the opt-in
+constexpr int kMaxCluster = 8;
+constexpr int kAhead = 8;         // logits of a thread in flight
 constexpr int kMinSlice = 4096;   // tokens per CTA that are worth a CTA
 constexpr u64 kAll = 1ull << 32;  // the smallest key of a logit that is not NaN
 
 struct Shared {
-  double exp2_64[64];                         // 2^(j/64)
+  double exp2_256[256];                       // 2^(j/256)
   uint32_t cnt[kBins], lo[kBins], hi[kBins];  // this CTA's bins; masses as 64 bits in halves
   uint32_t g_cnt[kBins];                      // rank 0: the row's bins
   u64 g_mass[kBins];
   // rank 0: the list, in order of arrival, then ranked (by key, later by index)
-  __align__(16) u64 cand[kCand];
+  u64 cand[kCand];
   u64 sorted[kCand];
-  __align__(16) uint32_t place[kCand];
   u64 warp_mass[kWarps], warp_best[kWarps];
   uint32_t warp_cnt[kWarps];
-  u64 best, mass;   // this CTA's largest key, kept mass
+  // every CTA's largest key, tokens sent to the list and kept mass, in every CTA
+  u64 best_of[kMaxCluster], mass_of[kMaxCluster];
+  int sent_of[kMaxCluster];
   int n_cand;       // rank 0
   // a pass's result, written to every CTA by rank 0
   int bin;
-  uint32_t bin_cnt, above_cnt;
+  uint32_t bin_cnt, above_cnt, total_cnt;
+  int sent;  // tokens of this CTA for the list
   u64 above_mass, target, cut;
 };
 
@@ -82,33 +87,39 @@ __device__ __forceinline__ u64 fraction_of(float f, u64 m, bool up) {
 
 struct Weights {
   float top;           // the row's largest logit
-  double octaves;      // 64 log2(e) / T: (x - top) in 64ths of an octave
+  double octaves;      // 256 log2(e) / T: (x - top) in 256ths of an octave
   double scale;        // mass of w = 1
   int mass_bits;       // its power of two
   const double *table;
 
-  // w of a logit that is not NaN, to 2^-44: with y = 64 log2 w split into an
-  // integer k and |f| <= 1/2, w = 2^(k >> 6) 2^((k & 63) / 64) e^r for r = f ln2 / 64,
-  // e^r by its series to r^4 (r^5 / 120 < 2^-44).  (Table look-up and a short
-  // series: P. T. P. Tang, ACM TOMS 15(2), 1989.)
+  __device__ __forceinline__ void set(float top_, float temperature, int bits, const double *t) {
+    top = top_;
+    octaves = 369.3299304675746 / (double)temperature;
+    mass_bits = bits;
+    scale = (double)(1ull << bits);
+    table = t;
+  }
+  // w of a logit that is not NaN, to 2^-42: with y = 256 log2 w split into an
+  // integer k and |f| <= 1/2, w = 2^(k >> 8) 2^((k & 255) / 256) e^r for
+  // r = f ln2 / 256, e^r by its series to r^3 (r^4 / 24 < 2^-42).  (Table look-up and
+  // a short series: P. T. P. Tang, ACM TOMS 15(2), 1989.)
   __device__ __forceinline__ double w(float x) const { return w_scaled(x, 0); }
   // w 2^bits
   __device__ __forceinline__ double w_scaled(float x, int bits) const {
     if (top == INFINITY) return x == INFINITY ? (bits ? scale : 1.0) : 0.0;
     if (x == -INFINITY) return 0.0;
     constexpr double kMagic = 6755399441055744.0;  // 1.5 2^52: the sum's low word is round(y)
-    constexpr double kC = 0.010830424696249145;    // ln2 / 64
-    const double y = fmax(((double)x - (double)top) * octaves, -60000.0);
+    constexpr double kC = 0.0027076061740622863;   // ln2 / 256
+    const double y = fmax(((double)x - (double)top) * octaves, -240000.0);  // below: no mass
     const double kd = y + kMagic;
     const int k = __double2loint(kd);
     const double f = y - (kd - kMagic);
-    double e = fma(f, kC * kC * kC * kC / 24, kC * kC * kC / 6);
-    e = fma(f, e, kC * kC / 2);
+    double e = fma(f, kC * kC * kC / 6, kC * kC / 2);
     e = fma(f, e, kC);
     e *= f;
-    const double t = table[k & 63];
+    const double t = table[k & 255];
     const double v = fma(t, e, t);
-    return __hiloint2double(__double2hiint(v) + (((k >> 6) + bits) << 20), __double2loint(v));
+    return __hiloint2double(__double2hiint(v) + (((k >> 8) + bits) << 20), __double2loint(v));
   }
   // round(w 2^mass_bits), below 2^51
   __device__ __forceinline__ u64 mass(float x) const {
@@ -141,6 +152,12 @@ __device__ __forceinline__ u64 before_warp(const u64 *v, u64 &total) {
 }
 static_assert(kWarps == 32, "a lane per warp");
 
+// the bin of a logit that is not NaN, `top` the largest: rising as the logit falls
+__device__ __forceinline__ int value_bin(float v, float top, float scale) {
+  if (v == top) return 0;
+  return (int)fminf((top - v) * scale, (float)(kBins - 1));
+}
+
 struct Row {
   cg::cluster_group cl;
   Shared &s;
@@ -148,15 +165,20 @@ struct Row {
   int base, len;   // the slice's first token and length
   int rank, ctas;
 
+  // whether token i of the slice, of logit v, is at or above a cut in the row's order
+  __device__ __forceinline__ bool keeps(float v, int i, u64 cut) const {
+    const float c = cut == kAll ? -INFINITY : order_value((uint32_t)(cut >> 32));
+    return v > c || (v == c && token_key(v, base + i) >= cut);
+  }
   template <class F>
   __device__ __forceinline__ void each(F f) {
     int i = threadIdx.x;
-    for (; i + 3 * kThreads < len; i += 4 * kThreads) {
-      float v[4];
+    for (; i + (kAhead - 1) * kThreads < len; i += kAhead * kThreads) {
+      float v[kAhead];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = x[i + k * kThreads];
+      for (int k = 0; k < kAhead; ++k) v[k] = x[i + k * kThreads];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) f(v[k], i + k * kThreads);
+      for (int k = 0; k < kAhead; ++k) f(v[k], i + k * kThreads);
     }
     for (; i < len; i += kThreads) f(x[i], i);
   }
@@ -176,6 +198,64 @@ struct Row {
     uint32_t hi = (uint32_t)(m >> 32);
     if (atomicAdd(&s.lo[bin], lo) + lo < lo) ++hi;  // carry
     if (hi) atomicAdd(&s.hi[bin], hi);
+  }
+
+  // The first of the given bins at which the running count reaches k (k > 0) or the
+  // running mass (k == 0) the target; see find().  The result lands in this CTA's s.bin
+  // and beside it.
+  __device__ void locate(const uint32_t *cnt, const u64 *mass, uint32_t k, float top_p,
+                         uint32_t first_cnt, u64 first_mass) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int kPer = kBins / kThreads;
+    uint32_t c[kPer], csum = 0;
+    u64 m[kPer], msum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      c[i] = cnt[threadIdx.x * kPer + i];
+      m[i] = mass ? mass[threadIdx.x * kPer + i] : 0;
+      csum += c[i];
+      msum += m[i];
+    }
+    uint32_t cin = csum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t cu = __shfl_up_sync(0xffffffffu, cin, o);
+      if (lane >= o) cin += cu;
+    }
+    const u64 min_ = warp_scan64(msum);
+    if (lane == 31) {
+      s.warp_cnt[warp] = cin;
+      s.warp_mass[warp] = min_;
+    }
+    if (threadIdx.x == 0) s.bin = -1;
+    __syncthreads();
+    u64 total;
+    u64 mb = first_mass + before_warp(s.warp_mass, total) + min_ - msum;
+    total += first_mass;
+    uint32_t cw = s.warp_cnt[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t cu = __shfl_up_sync(0xffffffffu, cw, o);
+      if (lane >= o) cw += cu;
+    }
+    uint32_t cb = first_cnt + __shfl_sync(0xffffffffu, cw, warp) - s.warp_cnt[warp] + cin - csum;
+    if (threadIdx.x == kThreads - 1) s.total_cnt = cb + csum;
+    u64 target = s.target;
+    if (top_p == top_p) target = max(fraction_of(fmaxf(top_p, 0.f), total, true), 1ull);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const bool here = k ? (cb < k && cb + c[i] >= k) : (mb < target && mb + m[i] >= target);
+      if (here) {
+        s.bin = threadIdx.x * kPer + i;
+        s.bin_cnt = c[i];
+        s.above_cnt = cb;
+        s.above_mass = mb;
+        s.target = target;
+      }
+      cb += c[i];
+      mb += m[i];
+    }
+    __syncthreads();
   }
 
   // Sum the CTAs' bins and find the first at which the running count reaches
@@ -208,56 +288,7 @@ struct Row {
     else
       __syncthreads();
     if (rank == 0) {
-      const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-      constexpr int kPer = kBins / kThreads;
-      uint32_t c[kPer], csum = 0;
-      u64 m[kPer], msum = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        c[i] = s.g_cnt[threadIdx.x * kPer + i];
-        m[i] = s.g_mass[threadIdx.x * kPer + i];
-        csum += c[i];
-        msum += m[i];
-      }
-      uint32_t cin = csum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t cu = __shfl_up_sync(0xffffffffu, cin, o);
-        if (lane >= o) cin += cu;
-      }
-      const u64 min_ = warp_scan64(msum);
-      if (lane == 31) {
-        s.warp_cnt[warp] = cin;
-        s.warp_mass[warp] = min_;
-      }
-      if (threadIdx.x == 0) s.bin = -1;
-      __syncthreads();
-      u64 total;
-      u64 mb = first_mass + before_warp(s.warp_mass, total) + min_ - msum;
-      total += first_mass;
-      uint32_t cw = s.warp_cnt[lane];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t cu = __shfl_up_sync(0xffffffffu, cw, o);
-        if (lane >= o) cw += cu;
-      }
-      uint32_t cb = first_cnt + __shfl_sync(0xffffffffu, cw, warp) - s.warp_cnt[warp] + cin - csum;
-      u64 target = s.target;
-      if (top_p == top_p) target = max(fraction_of(fmaxf(top_p, 0.f), total, true), 1ull);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const bool here = k ? (cb < k && cb + c[i] >= k) : (mb < target && mb + m[i] >= target);
-        if (here) {
-          s.bin = threadIdx.x * kPer + i;
-          s.bin_cnt = c[i];
-          s.above_cnt = cb;
-          s.above_mass = mb;
-          s.target = target;
-        }
-        cb += c[i];
-        mb += m[i];
-      }
-      __syncthreads();
+      locate(s.g_cnt, s.g_mass, k, top_p, first_cnt, first_mass);
       if (threadIdx.x > 0 && threadIdx.x < ctas) {
         Shared *o = cl.map_shared_rank(&s, threadIdx.x);
         o->bin = s.bin;
@@ -271,6 +302,65 @@ struct Row {
       cl.sync();
     else
       __syncthreads();
+  }
+
+  // The slice's tokens with keys >= within into the bins.  The last bin also takes all
+  // that lies below the range: summed in registers first, as half the row may fall
+  // there.
+  template <class M>
+  __device__ __forceinline__ void fill_bins(u64 within, float top, float scale, M mass) {
+    uint32_t rest_n = 0;
+    u64 rest_m = 0;
+    each([&](float v, int i) {
+      if (!keeps(v, i, within)) return;
+      const u64 m = mass(v);
+      const int bin = value_bin(v, top, scale);
+      if (bin < kBins - 1) {
+        add(bin, 1, m);
+      } else {
+        ++rest_n;
+        rest_m += m;
+      }
+    });
+    rest_n = __reduce_add_sync(0xffffffffu, rest_n);
+    rest_m = warp_sum64(rest_m);
+    if ((threadIdx.x & 31) == 0) add(kBins - 1, rest_n, rest_m);
+  }
+
+  // the bins of one value per thread (NaN: none)
+  __device__ __forceinline__ void fill_bins_with(float v, float top, float scale) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.cnt[i] = 0;
+    __syncthreads();
+    if (v == v) atomicAdd(&s.cnt[value_bin(v, top, scale)], 1u);
+    __syncthreads();
+  }
+
+  // For a short top-k: the slice's first k tokens, and few more, into rank 0's list,
+  // their number into s.sent.  The k-th largest of the threads' own maxima is not above
+  // the slice's k-th largest, and few other tokens exceed it: so its bin, found among
+  // one value per thread, bounds what is sent.  `mine`: this thread's maximum (NaN: no
+  // token), `top`: the slice's.
+  __device__ void send_first(uint32_t k, float mine, float top, float scale) {
+    fill_bins_with(mine, top, scale);
+    locate(s.cnt, nullptr, k, NAN, 0, 0);
+    const int last = s.bin < 0 ? kBins - 1 : s.bin;
+    auto sends = [&](float v) {
+      return v == top || (top - v) * scale < (float)(last + 1) || (last == kBins - 1 && v == v);
+    };
+    each([&](float v, int i) {  // first into a list of this CTA's own
+      if (!sends(v)) return;
+      const int at = atomicAdd(&s.sent, 1);
+      if (at < kCand) s.sorted[at] = token_key(v, base + i);
+    });
+    __syncthreads();
+    if (ctas > 1) cl.barrier_wait();  // the row's CTAs have started
+    const int n = s.sent;
+    if (n > kCand) return;
+    if (threadIdx.x == 0) s.bin = atomicAdd(cl.map_shared_rank(&s.n_cand, 0), n);
+    __syncthreads();
+    const int at = s.bin + threadIdx.x;
+    if (threadIdx.x < n && at < kCand)
+      *cl.map_shared_rank(&s.cand[at], 0) = s.sorted[threadIdx.x];
   }
 
   // tokens of `pred` into rank 0's list, in any order
@@ -288,23 +378,40 @@ struct Row {
       __syncthreads();
   }
 
-  // rank 0: the list in order of falling keys into s.sorted.  A token's place is
-  // the number of larger keys, counted by as many threads as the block has to spare.
-  __device__ void rank_list(int n) {
-    int share = 1;
-    while (2 * share * n <= kThreads) share *= 2;
-    for (int i = threadIdx.x; i < n; i += kThreads) s.place[i] = 0;
-    __syncthreads();
-    for (int t = threadIdx.x; t < n * share; t += kThreads) {
-      const int i = t / share, j0 = t - i * share;
-      const u64 key = s.cand[i];
-      uint32_t c = 0;
+  // rank 0: the list in order of falling keys into s.sorted: a short one by counting
+  // larger keys, else a bitonic sort, a key per thread, by shuffles within a warp and
+  // through shared memory across warps.
+  __device__ void sort_list(int n) {
+    const int i = threadIdx.x;
+    u64 key = i < n ? s.cand[i] : 0;
+    if (n <= 128) {
+      int place = 0;
+      if (i < n)
 #pragma unroll 4
-      for (int j = j0; j < n; j += share) c += s.cand[j] > key;
-      if (c) atomicAdd(&s.place[i], c);
+        for (int j = 0; j < n; ++j) place += s.cand[j] > key;
+      if (i < n) s.sorted[place] = key;
+      __syncthreads();
+      return;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) s.sorted[s.place[i]] = s.cand[i];
+    int size = 32;
+    while (size < n) size *= 2;
+    for (int k = 2; k <= size; k *= 2) {
+      for (int j = k / 2; j > 0; j /= 2) {
+        u64 other;
+        if (j >= 32) {
+          if (i < size) s.sorted[i] = key;
+          __syncthreads();
+          other = i < size ? s.sorted[i ^ j] : 0;
+          __syncthreads();
+        } else {
+          other = __shfl_xor_sync(0xffffffffu, key, j);
+        }
+        // falling runs where bit k of the index is 0
+        const bool larger = ((i & k) == 0) == ((i & j) == 0);
+        key = larger ? max(key, other) : min(key, other);
+      }
+    }
+    if (i < size) s.sorted[i] = key;
     __syncthreads();
   }
 
@@ -314,45 +421,24 @@ struct Row {
   // down to the cut's bin fit the list, they are left there instead (*listed set).
   __device__ u64 cut(uint32_t k, float top_p, u64 within, const Weights &W, float bin_scale,
                      bool *listed) {
-    auto value_bin = [&](float v) {
-      if (v == W.top) return 0;
-      return (int)fminf((W.top - v) * bin_scale, (float)(kBins - 1));
-    };
     clear_bins(!k);
-    {
-      // the last bin also takes all that lies below the range: summed in
-      // registers first, as half the row may fall there
-      uint32_t rest_n = 0;
-      u64 rest_m = 0;
-      each([&](float v, int i) {
-        const u64 key = token_key(v, base + i);
-        if (key < within) return;
-        const u64 m = k ? 0 : W.mass(v);
-        const int bin = value_bin(v);
-        if (bin < kBins - 1) {
-          add(bin, 1, m);
-        } else {
-          ++rest_n;
-          rest_m += m;
-        }
-      });
-      rest_n = __reduce_add_sync(0xffffffffu, rest_n);
-      rest_m = warp_sum64(rest_m);
-      if ((threadIdx.x & 31) == 0) add(kBins - 1, rest_n, rest_m);
-    }
+    fill_bins(within, W.top, bin_scale, [&](float v) { return k ? 0 : W.mass(v); });
     find(k, top_p, 0, 0);
     if (s.bin < 0) return within;  // fewer than k tokens: all of them
     const int vbin = s.bin;
     if (listed && s.above_cnt + s.bin_cnt <= kCand) {
       *listed = true;
-      gather([&](float v, u64 key) { return key >= within && value_bin(v) <= vbin; });
+      gather([&](float v, u64 key) {
+        return key >= within && value_bin(v, W.top, bin_scale) <= vbin;
+      });
       return within;
     }
     // narrow a crowded bin by digits of the key, highest first
     int shift = 64, bits = 0;
     u64 prefix = 0;
     auto inside = [&](float v, u64 key) {
-      return key >= within && value_bin(v) == vbin && (shift == 64 || (key >> shift) == prefix);
+      return key >= within && value_bin(v, W.top, bin_scale) == vbin &&
+             (shift == 64 || (key >> shift) == prefix);
     };
     while (s.bin_cnt > kCand) {
       bits = min(11, shift);
@@ -372,7 +458,7 @@ struct Row {
     gather(inside);
     if (rank == 0) {
       const int n = s.n_cand;
-      rank_list(n);
+      sort_list(n);
       if (k) {
         if (threadIdx.x == 0) s.cut = s.sorted[k - s.above_cnt - 1];
       } else if (threadIdx.x < 32) {
@@ -405,10 +491,22 @@ struct Row {
   // rank 0: both cuts and the draw on the list.  top_p_target: the mass the top-p
   // prefix has to reach, or 0 to take the share of the first k tokens' mass.
   __device__ void draw_listed(uint32_t k, float top_p, u64 top_p_target, double min_w, float u,
-                              const Weights &W, int32_t *token, float *prob) {
+                              const Weights &W, float bin_scale, int32_t *token, float *prob) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = threadIdx.x;
-    const int n = s.n_cand;
-    rank_list(n);
+    int n = s.n_cand;
+    if (k && n > 128) {  // slices' lists joined: down to the bin of the k-th
+      const u64 key = i < n ? s.cand[i] : 0;
+      const float v = i < n ? order_value((uint32_t)(key >> 32)) : NAN;
+      fill_bins_with(v, W.top, bin_scale);
+      locate(s.cnt, nullptr, k, NAN, 0, 0);
+      if (threadIdx.x == 0) s.n_cand = 0;
+      __syncthreads();
+      if (i < n && (s.bin < 0 || value_bin(v, W.top, bin_scale) <= s.bin))
+        s.cand[atomicAdd(&s.n_cand, 1)] = key;
+      __syncthreads();
+      n = s.n_cand;
+    }
+    sort_list(n);
     const int n_k = k ? min(n, (int)k) : n;
     const u64 key = i < n_k ? s.sorted[i] : 0;
     const float v = order_value((uint32_t)(key >> 32));
@@ -427,7 +525,7 @@ struct Row {
       s.g_mass[i] = m;
     }
     __syncthreads();
-    rank_list(n_keep);
+    sort_list(n_keep);
     const uint32_t at = i < n_keep ? (uint32_t)s.sorted[i] & (kCand - 1) : 0;
     const u64 mine = i < n_keep ? s.g_mass[at] : 0;
     in = warp_scan64(mine);
@@ -453,10 +551,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(
   extern __shared__ __align__(16) uint8_t s_raw[];
   Shared &s = *reinterpret_cast<Shared *>(s_raw);
   float *s_x = reinterpret_cast<float *>(s_raw + sizeof(Shared));
-  if (threadIdx.x < 64) s.exp2_64[threadIdx.x] = exp2(threadIdx.x / 64.0);
-  pdl_wait_then_release();
   cg::cluster_group cl = cg::this_cluster();
   const int rank = cl.block_rank(), ctas = cl.num_blocks();
+  if (threadIdx.x == 0) s.n_cand = s.sent = 0;
+  if (threadIdx.x < 256) s.exp2_256[threadIdx.x] = exp2(threadIdx.x / 256.0);
+  pdl_wait_then_release();
+  __syncthreads();
+  if (ctas > 1) cl.barrier_arrive();
   const int row = blockIdx.x / ctas;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int base = min(n, rank * slice), len = min(n - base, slice);
@@ -464,27 +565,69 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(
   const mlm_sample_params p = params[row];
   Row r{cl, s, g, base, len, rank, ctas};
 
-  // the slice into shared memory; the row's largest key
-  u64 best = 0;
+  // the slice into shared memory; its largest logit, the first of equals
+  float mine = -INFINITY;
+  int mine_at = -1;
   r.each([&](float v, int i) {
     if (resident) s_x[i] = v;
-    const u64 key = token_key(v, base + i);
-    best = key > best ? key : best;
+    if (v > mine) {
+      mine = v;
+      mine_at = i;
+    }
   });
   if (resident) r.x = s_x;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if (lane == 0) s.warp_best[warp] = best;
+  u64 best = mine_at < 0 ? 0 : token_key(mine, base + mine_at);
+  {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+    if (lane == 0) s.warp_best[warp] = ((u64)hi << 32) | lo;
+  }
   __syncthreads();
   best = s.warp_best[lane];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+    best = ((u64)hi << 32) | lo;
+  }
+  if (best < kAll) {  // nothing above -inf: the first -inf, if there is one
+    uint32_t first = 0;
+    r.each([&](float v, int i) {
+      if (v == -INFINITY) first = max(first, ~(uint32_t)(base + i));
+    });
+    first = __reduce_max_sync(0xffffffffu, first);
+    __syncthreads();
+    if (lane == 0) s.warp_best[warp] = first;
+    __syncthreads();
+    first = __reduce_max_sync(0xffffffffu, (uint32_t)s.warp_best[lane]);
+    best = first ? ((u64)order_bits(-INFINITY) << 32) | first : 0;
+  }
+
+  // bins over the logits that matter: 24 temperatures, but at least 16 and at
+  // most 64 below the largest
+  const float bin_scale = (float)kBins / fminf(fmaxf(24.f * p.temperature, 16.f), 64.f);
+  const uint32_t k = p.top_k > 0 && p.top_k < n ? (uint32_t)p.top_k : 0;
+  // half the list for the slices' first k, the rest for what shares their last bins
+  const bool is_short = k && 2 * (u64)k * ctas <= kCand && p.temperature > 0.f;
+  if (is_short && best >= kAll)
+    r.send_first(k, mine_at < 0 ? NAN : mine, order_value((uint32_t)(best >> 32)), bin_scale);
+  else if (ctas > 1)
+    cl.barrier_wait();
+  int sent = 0;
   if (ctas > 1) {
-    if (threadIdx.x == 0) s.best = best;
+    __syncthreads();
+    if (threadIdx.x < ctas) {
+      Shared *o = cl.map_shared_rank(&s, threadIdx.x);
+      o->best_of[rank] = best;
+      o->sent_of[rank] = s.sent;
+    }
     cl.sync();
-    best = *cl.map_shared_rank(&s.best, lane < ctas ? lane : 0);
+    best = s.best_of[lane < ctas ? lane : 0];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    sent = __reduce_add_sync(0xffffffffu, lane < ctas ? s.sent_of[lane] : 0);
+  } else {
+    __syncthreads();
+    sent = s.sent;
   }
 
   const float top = order_value((uint32_t)(best >> 32));
@@ -495,35 +638,27 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(
       token[row] = best < kAll ? 0 : (int32_t)~(uint32_t)best;
       if (prob) prob[row] = none ? 0.f : 1.f;
     }
-    cl.sync();  // no CTA leaves while another may still read its s.best
     return;
   }
   Weights W;
-  W.top = top;
-  W.octaves = 92.332482616893656 / (double)p.temperature;  // 64 log2(e) / T
-  W.scale = (double)(1ull << mass_bits);
-  W.mass_bits = mass_bits;
-  W.table = s.exp2_64;
-  // bins over the logits that matter: 24 temperatures, but at least 16 and at
-  // most 64 below the largest
-  const float bin_scale = (float)kBins / fminf(fmaxf(24.f * p.temperature, 16.f), 64.f);
-  const uint32_t k = p.top_k > 0 && p.top_k < n ? (uint32_t)p.top_k : 0;
+  W.set(top, p.temperature, mass_bits, s.exp2_256);
   const double min_w = p.min_p > 0.f ? fmin((double)p.min_p, 1.0) : 0.0;
   float u = uniform[row];
   u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;  // NaN: 0
   u64 cut = kAll;
-  bool listed = false;
-  if (k) cut = r.cut(k, NAN, cut, W, bin_scale, &listed);
+  bool listed = is_short && sent <= kCand;
+  if (k && !listed) cut = r.cut(k, NAN, cut, W, bin_scale, &listed);
   if (p.top_p < 1.f && !listed) cut = r.cut(0, p.top_p, cut, W, bin_scale, k ? nullptr : &listed);
   if (listed) {
     if (rank == 0)
-      r.draw_listed(k, p.top_p, k ? 0 : s.target, min_w, u, W, token + row, prob ? prob + row : nullptr);
-    return;  // the other CTAs' shared memory is no longer read (gather ended in a barrier)
+      r.draw_listed(k, p.top_p, k ? 0 : s.target, min_w, u, W, bin_scale, token + row,
+                    prob ? prob + row : nullptr);
+    return;  // nothing of this CTA's shared memory is read any more
   }
 
   // the kept mass of every warp's stretch
   auto kept = [&](float v, int i) -> u64 {
-    if (token_key(v, base + i) < cut) return 0;
+    if (!r.keeps(v, i, cut)) return 0;
     return min_w == 0.0 || W.w(v) >= min_w ? W.mass(v) : 0;
   };
   // this warp's share of a range, 4 loads in flight
@@ -547,9 +682,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(
   u64 total;
   u64 before = before_warp(s.warp_mass, total);
   if (ctas > 1) {
-    if (threadIdx.x == 0) s.mass = total;
+    if (threadIdx.x < ctas) cl.map_shared_rank(&s, threadIdx.x)->mass_of[rank] = total;
     cl.sync();
-    const u64 of = lane < ctas ? *cl.map_shared_rank(&s.mass, lane) : 0;
+    const u64 of = lane < ctas ? s.mass_of[lane] : 0;
     const u64 in = warp_scan64(of);
     total = __shfl_sync(0xffffffffu, in, 31);
     before += __shfl_sync(0xffffffffu, in - of, rank);
@@ -589,7 +724,6 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(
       }
     }
   }
-  if (ctas > 1) cl.sync();  // no CTA leaves while another may still read its s.mass
 }
 
 constexpr int kMaxN = 1 << 22;
@@ -602,8 +736,6 @@ static_assert(sizeof(Shared) + kSliceBytes <= 227 * 1024, "a CTA's shared memory
 int sample_init(mlm_ctx *ctx) {
   MLM_CUDA_TRY(ctx, cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)(sizeof(Shared) + kSliceBytes)));
-  MLM_CUDA_TRY(ctx, cudaFuncSetAttribute(sample_kernel,
-                                         cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   return MLM_OK;
 }
 
@@ -625,7 +757,8 @@ extern "C" int mlm_sample_f32(mlm_ctx *ctx, const float *logits, int rows, int n
               MLM_ERR_ALIGN, "mlm_sample_f32: buffers must be 4-byte aligned");
   DeviceGuard guard(ctx);
   int ctas = kMaxCluster;
-  while (ctas > 1 && (rows * ctas > ctx->sm_count || n < kMinSlice * ctas)) ctas /= 2;
+  // twice the SMs' number of CTAs: rows of different settings take different times
+  while (ctas > 1 && (rows * ctas > 2 * ctx->sm_count || n < kMinSlice * ctas)) ctas /= 2;
   const int slice = (n + ctas - 1) / ctas;
   const int resident = (size_t)slice * 4 <= kSliceBytes;
   int bits = 62;
