@@ -600,6 +600,13 @@ int mlm_llama_prefill(mlm_llama *m, const int32_t *tokens, int n, float *logits,
  * other capture on ctx's stream). */
 int mlm_llama_decode_greedy(mlm_llama *m, int token, int steps, int32_t *tokens_out_dev);
 
+/* Sampled generation: mlm_llama_decode_greedy with mlm_sample_f32 in the argmax's
+ * place.  `params` (host) holds the settings, uniforms_dev[i] (device, [steps]) the
+ * i-th step's random number.  The settings and numbers are copied into the runner;
+ * a call with others replays the same captured step. */
+int mlm_llama_decode_sample(mlm_llama *m, int token, int steps, const mlm_sample_params *params,
+                            const float *uniforms_dev, int32_t *tokens_out_dev);
+
 /* A batch of independent sequences on one runner (the reference decodes one
  * conversation at a time).  mlm_llama_create_batch allocates `batch`
  * (1 .. min(64, max_seq)) sets of KV caches; the calls above act on
@@ -625,6 +632,11 @@ int mlm_llama_prefill_seq(mlm_llama *m, int seq, const int32_t *tokens, int n, f
 int mlm_llama_seq_position(const mlm_llama *m, int seq);
 int mlm_llama_forward_batch(mlm_llama *m, const int32_t *tokens, float *logits);
 int mlm_llama_decode_greedy_batch(mlm_llama *m, const int32_t *tokens, int steps,
+                                  int32_t *tokens_out_dev);
+/* The batch's sampled generation: params (host) one per sequence, uniforms_dev
+ * (device) [steps][batch]. */
+int mlm_llama_decode_sample_batch(mlm_llama *m, const int32_t *tokens, int steps,
+                                  const mlm_sample_params *params, const float *uniforms_dev,
                                   int32_t *tokens_out_dev);
 
 #ifdef __cplusplus

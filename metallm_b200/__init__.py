@@ -424,6 +424,26 @@ class Llama:
                                                          ctypes.c_void_p(int(tokens_out))),
                     "mlm_llama_decode_greedy")
 
+    def decode_sample(self, token: int, steps: int, params: tuple, uniforms, tokens_out) -> None:
+        """`steps` sampled steps; params (temperature, top_k, top_p, min_p), uniforms
+        fp32 [steps] on the device."""
+        p = sample_params([params])
+        self._check(self.ctx.lib.mlm_llama_decode_sample(
+            self.handle, token, steps, p.ctypes.data, ctypes.c_void_p(int(uniforms)),
+            ctypes.c_void_p(int(tokens_out))), "mlm_llama_decode_sample")
+
+    def decode_sample_batch(self, tokens: Sequence[int], steps: int, params: Sequence[tuple],
+                            uniforms, tokens_out) -> None:
+        """`steps` sampled steps of every sequence; params one per sequence, uniforms fp32
+        and tokens_out int32 [steps][batch] on the device."""
+        arr = (ctypes.c_int32 * self.batch)(*[int(t) for t in tokens])
+        p = sample_params(params)
+        if len(p) != self.batch:
+            raise ValueError(f"{len(p)} settings for {self.batch} sequences")
+        self._check(self.ctx.lib.mlm_llama_decode_sample_batch(
+            self.handle, arr, steps, p.ctypes.data, ctypes.c_void_p(int(uniforms)),
+            ctypes.c_void_p(int(tokens_out))), "mlm_llama_decode_sample_batch")
+
     def close(self) -> None:
         if self.handle and self.ctx.handle:
             self.ctx.lib.mlm_llama_destroy(self.handle)

@@ -178,6 +178,8 @@ SIGNATURES = [
     ("mlm_llama_seq_position", c_int, [c_vp, c_int]),
     ("mlm_llama_forward_batch", c_int, [c_vp, c_vp, c_vp]),
     ("mlm_llama_decode_greedy_batch", c_int, [c_vp, c_vp, c_int, c_vp]),
+    ("mlm_llama_decode_sample", c_int, [c_vp, c_int, c_int, c_vp, c_vp, c_vp]),
+    ("mlm_llama_decode_sample_batch", c_int, [c_vp, c_vp, c_int, c_vp, c_vp, c_vp]),
     ("mlm_tp_unique_id", c_int, [c_vp, c_vp, c_size]),
     ("mlm_tp_init", c_int, [c_vp, c_int, c_int, c_vp]),
     ("mlm_tp_info", c_int, [c_vp, ctypes.POINTER(c_int), ctypes.POINTER(c_int)]),

@@ -51,9 +51,6 @@ __device__ __forceinline__ float2 unpack_f16(uint32_t v) {
 __device__ __forceinline__ float low_f16(uint32_t v) {
   return __half2float(__ushort_as_half((unsigned short)v));
 }
-__device__ __forceinline__ float high_f16(uint32_t v) {
-  return __half2float(__ushort_as_half((unsigned short)(v >> 16)));
-}
 __device__ __forceinline__ uint32_t u4_get(const uint4 &v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }

@@ -142,6 +142,12 @@ struct mlm_llama {
   unsigned long long *b_keys_l = nullptr, *b_keys = nullptr;  // [batch], [tp][batch]
   cudaGraph_t bstep_graph = nullptr;
   cudaGraphExec_t bstep_exec = nullptr;
+  // sampled decoding: the settings per sequence, [max_seq][batch] random numbers, with
+  // TP the gathered logits of every row, and the captured steps
+  mlm_sample_params *s_params = nullptr;
+  float *s_uniform = nullptr, *s_logits = nullptr;
+  cudaGraph_t sstep_graph = nullptr, sbstep_graph = nullptr;
+  cudaGraphExec_t sstep_exec = nullptr, sbstep_exec = nullptr;
 
   size_t seq_elems() const { return (size_t)cfg.max_seq * kvdim(); }
   int position(int b) const { return b == 0 ? pos : seq_pos[b]; }
@@ -235,8 +241,23 @@ struct mlm_llama {
 
   // final norm, the output GEMV and the greedy token into state[kToken];
   // the full logits also land in lg_out when it is given
-  int head(const float *h, float *lg_out) {
+  // (`sampled`: a sampled token there instead, by s_params and the step's number)
+  int head(const float *h, float *lg_out, bool sampled = false) {
     int st;
+    if (sampled) {
+      if (tp_on) {
+        if ((st = gemv_t(output_type, output, vocab_l(), cfg.dim, normed(h, out_norm), logits_l,
+                         nullptr)))
+          return st;
+        if ((st = tp_allgather_bytes(ctx, logits_l, logits, sizeof(float) * vocab_l(), ctx->stream)))
+          return st;
+      } else if ((st = gemv_t(output_type, output, cfg.vocab, cfg.dim, normed(h, out_norm), logits,
+                              nullptr))) {
+        return st;
+      }
+      return sample_launch(ctx, logits, 1, cfg.vocab, cfg.vocab, s_params, s_uniform, state + kStep,
+                           state + kToken, nullptr, ctx->stream);
+    }
     if (!tp_on) {
       float *lg = lg_out ? lg_out : logits;
       if ((st = gemv_t(output_type, output, cfg.vocab, cfg.dim, normed(h, out_norm), lg, nullptr)))
@@ -259,7 +280,7 @@ struct mlm_llama {
   // embedding of state[kToken], all layers; then, when `with_head`, the
   // final norm, the output GEMV (logits into lg when given) and the argmax
   // into state[kToken]
-  int step(bool with_head, float *lg) {
+  int step(bool with_head, float *lg, bool sampled = false) {
     int st;
     if ((st = embed_launch(ctx, tok_embd, cfg.vocab, cfg.dim, state + kToken, hidden,
                            ctx->stream)))
@@ -267,7 +288,7 @@ struct mlm_llama {
     for (int l = 0; l < cfg.n_layers; ++l)
       if ((st = layer(l, hidden))) return st;
     if (!with_head) return MLM_OK;
-    return head(hidden, lg);
+    return head(hidden, lg, sampled);
   }
 
   // T prompt tokens (device ids in pf_tokens) at positions pos .. pos+T-1:
@@ -322,7 +343,8 @@ struct mlm_llama {
   // over the batch's B rows, attention per sequence over its own cache; the
   // greedy tokens land in tok_b; logits (all rows, [B][vocab]) in lg_out
   // when it is given
-  int step_batch(float *lg_out) {
+  // (`sampled`: sampled tokens instead, by s_params and the step's numbers)
+  int step_batch(float *lg_out, bool sampled = false) {
     const mlm_llama_config &c = cfg;
     cudaStream_t s = ctx->stream;
     const int B = batch;
@@ -360,6 +382,18 @@ struct mlm_llama {
       if ((st = rmsnorm_rows_bf16_launch(ctx, pf_hidden, out_norm, pf_x, B, c.dim, c.rms_eps, s)))
         return st;
       if ((st = linear(output, vocab_l(), c.dim, pf_x, B, b_logits, nullptr))) return st;
+    }
+    if (sampled) {
+      const float *rows = b_logits;
+      if (tp_on) {
+        for (int b = 0; b < B; ++b)
+          if ((st = tp_allgather_bytes(ctx, b_logits + (size_t)b * vocab_l(),
+                                       s_logits + (size_t)b * c.vocab, sizeof(float) * vocab_l(), s)))
+            return st;
+        rows = s_logits;
+      }
+      return sample_launch(ctx, rows, B, c.vocab, c.vocab, s_params, s_uniform, state + kStep, tok_b,
+                           nullptr, s);
     }
     for (int b = 0; b < B; ++b) {
       st = tp_on ? argmax_key_launch(ctx, b_logits + (size_t)b * vocab_l(), vocab_l(),
@@ -449,6 +483,10 @@ struct mlm_llama {
     if (step_graph) cudaGraphDestroy(step_graph);
     if (bstep_exec) cudaGraphExecDestroy(bstep_exec);
     if (bstep_graph) cudaGraphDestroy(bstep_graph);
+    if (sstep_exec) cudaGraphExecDestroy(sstep_exec);
+    if (sstep_graph) cudaGraphDestroy(sstep_graph);
+    if (sbstep_exec) cudaGraphExecDestroy(sbstep_exec);
+    if (sbstep_graph) cudaGraphDestroy(sbstep_graph);
     for (void *p : allocs) cudaFree(p);
     allocs.clear();
   }
@@ -582,7 +620,10 @@ static int llama_create(mlm_ctx *ctx, const mlm_llama_config *cfg, int batch,
         m->alloc(&m->gen_b, sizeof(int32_t) * c.max_seq * batch) ||
         m->alloc(&m->b_logits, sizeof(float) * batch * m->vocab_l()) ||
         m->alloc(&m->b_keys_l, sizeof(unsigned long long) * batch) ||
-        m->alloc(&m->b_keys, sizeof(unsigned long long) * batch * tp))
+        m->alloc(&m->b_keys, sizeof(unsigned long long) * batch * tp) ||
+        m->alloc(&m->s_params, sizeof(mlm_sample_params) * batch) ||
+        m->alloc(&m->s_uniform, sizeof(float) * c.max_seq * batch) ||
+        (m->tp_on && m->alloc(&m->s_logits, sizeof(float) * batch * c.vocab)))
       return fail(MLM_ERR_ALLOC);
     if (m->tp_on &&
         (m->alloc(&m->part, sizeof(float) * c.dim) ||
@@ -849,6 +890,114 @@ extern "C" int mlm_llama_decode_greedy_batch(mlm_llama *m, const int32_t *tokens
   }
   if ((st = m->set_state(0, 0, 0)) != MLM_OK) return st;
   for (int i = 0; i < steps; ++i) MLM_CUDA_TRY(ctx, cudaGraphLaunch(m->bstep_exec, ctx->stream));
+  MLM_CUDA_TRY(ctx, cudaMemcpyAsync(tokens_out, m->gen_b, sizeof(int32_t) * steps * m->batch,
+                                    cudaMemcpyDeviceToDevice, ctx->stream));
+  batch_advance(m, steps);
+  return MLM_OK;
+}
+
+// Captures one decode step as a graph (`enqueue` queues it); the graph is replayed for
+// every token.
+template <class F>
+static int capture_step(mlm_ctx *ctx, const char *what, cudaGraph_t *graph, cudaGraphExec_t *exec,
+                        F enqueue) {
+  MLM_CUDA_TRY(ctx, cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal));
+  const int st = enqueue();
+  cudaGraph_t g = nullptr;
+  const cudaError_t e = cudaStreamEndCapture(ctx->stream, &g);
+  if (st != MLM_OK || e != cudaSuccess) {
+    if (g) cudaGraphDestroy(g);
+    cudaGetLastError();
+    return st != MLM_OK ? st
+                        : set_error(ctx, MLM_ERR_CUDA, "%s: capture: %s", what, cudaGetErrorString(e));
+  }
+  cudaGraphExec_t x = nullptr;
+  const cudaError_t i = cudaGraphInstantiate(&x, g, 0);
+  if (i != cudaSuccess) {
+    cudaGraphDestroy(g);
+    cudaGetLastError();
+    return set_error(ctx, MLM_ERR_CUDA, "%s: instantiate: %s", what, cudaGetErrorString(i));
+  }
+  *graph = g;
+  *exec = x;
+  return MLM_OK;
+}
+
+// the settings and the steps' numbers into the runner's own buffers
+static int sample_begin(mlm_llama *m, const mlm_sample_params *params, const float *uniforms, int rows,
+                        int steps, const char *what) {
+  mlm_ctx *ctx = m->ctx;
+  MLM_REQUIRE(ctx, params && uniforms, MLM_ERR_ARG, "%s: no settings or random numbers", what);
+  MLM_REQUIRE(ctx, aligned4(uniforms), MLM_ERR_ALIGN, "%s: the random numbers must be 4-byte aligned",
+              what);
+  MLM_REQUIRE(ctx, m->cfg.vocab <= sample_max_n(), MLM_ERR_UNSUPPORTED, "%s: vocabulary %d (at most %d)",
+              what, m->cfg.vocab, sample_max_n());
+  MLM_CUDA_TRY(ctx, cudaMemcpyAsync(m->s_params, params, sizeof(mlm_sample_params) * rows,
+                                    cudaMemcpyHostToDevice, ctx->stream));
+  MLM_CUDA_TRY(ctx, cudaMemcpyAsync(m->s_uniform, uniforms, sizeof(float) * steps * rows,
+                                    cudaMemcpyDeviceToDevice, ctx->stream));
+  // the settings may lie in pageable host memory that the caller reuses
+  MLM_CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream));
+  return MLM_OK;
+}
+
+extern "C" int mlm_llama_decode_sample(mlm_llama *m, int token, int steps,
+                                       const mlm_sample_params *params, const float *uniforms,
+                                       int32_t *tokens_out) {
+  if (!m) return MLM_ERR_ARG;
+  mlm_ctx *ctx = m->ctx;
+  const char *what = "mlm_llama_decode_sample";
+  MLM_REQUIRE(ctx, tokens_out && steps > 0, MLM_ERR_ARG, "%s: no output", what);
+  MLM_REQUIRE(ctx, token >= 0 && token < m->cfg.vocab, MLM_ERR_ARG, "%s: invalid token id %d", what,
+              token);
+  MLM_REQUIRE(ctx, steps <= m->cfg.max_seq - m->pos, MLM_ERR_STATE,
+              "%s: %d steps at position %d exceed the cache (%d)", what, steps, m->pos,
+              m->cfg.max_seq);
+  int st = sample_begin(m, params, uniforms, 1, steps, what);
+  if (st != MLM_OK) return st;
+  if (!m->sstep_exec &&
+      (st = capture_step(ctx, what, &m->sstep_graph, &m->sstep_exec, [&] {
+         const int s = m->step(true, nullptr, true);
+         return s != MLM_OK ? s
+                            : check_launch_pdl(ctx,
+                                               launch_pdl(advance_kernel, dim3(1), dim3(1), 0,
+                                                          ctx->stream, m->state, m->gen_tokens),
+                                               what);
+       })) != MLM_OK)
+    return st;
+  if ((st = m->set_state(token, m->pos, 0)) != MLM_OK) return st;
+  for (int i = 0; i < steps; ++i) MLM_CUDA_TRY(ctx, cudaGraphLaunch(m->sstep_exec, ctx->stream));
+  MLM_CUDA_TRY(ctx, cudaMemcpyAsync(tokens_out, m->gen_tokens, sizeof(int32_t) * steps,
+                                    cudaMemcpyDeviceToDevice, ctx->stream));
+  m->pos += steps;
+  return MLM_OK;
+}
+
+extern "C" int mlm_llama_decode_sample_batch(mlm_llama *m, const int32_t *tokens, int steps,
+                                             const mlm_sample_params *params, const float *uniforms,
+                                             int32_t *tokens_out) {
+  if (!m) return MLM_ERR_ARG;
+  mlm_ctx *ctx = m->ctx;
+  const char *what = "mlm_llama_decode_sample_batch";
+  MLM_REQUIRE(ctx, tokens_out && steps > 0 && steps <= m->cfg.max_seq, MLM_ERR_ARG,
+              "%s: no output, or steps=%d", what, steps);
+  int st = batch_begin(m, tokens, steps, what);
+  if (st == MLM_OK) st = sample_begin(m, params, uniforms, m->batch, steps, what);
+  if (st != MLM_OK) return st;
+  if (!m->sbstep_exec &&
+      (st = capture_step(ctx, what, &m->sbstep_graph, &m->sbstep_exec, [&] {
+         const int s = m->step_batch(nullptr, true);
+         return s != MLM_OK
+                    ? s
+                    : check_launch_pdl(ctx,
+                                       launch_pdl(advance_batch_kernel, dim3(1), dim3(64), 0,
+                                                  ctx->stream, m->state, m->pos_b, m->tok_b, m->gen_b,
+                                                  m->batch),
+                                       what);
+       })) != MLM_OK)
+    return st;
+  if ((st = m->set_state(0, 0, 0)) != MLM_OK) return st;
+  for (int i = 0; i < steps; ++i) MLM_CUDA_TRY(ctx, cudaGraphLaunch(m->sbstep_exec, ctx->stream));
   MLM_CUDA_TRY(ctx, cudaMemcpyAsync(tokens_out, m->gen_b, sizeof(int32_t) * steps * m->batch,
                                     cudaMemcpyDeviceToDevice, ctx->stream));
   batch_advance(m, steps);

@@ -73,7 +73,13 @@ int set_error(mlm_ctx *ctx, int code, const char *fmt, ...)
     __attribute__((format(printf, 3, 4)));
 int check_launch(mlm_ctx *ctx, const char *what);
 int kv4_attn_init(mlm_ctx *ctx);  // kv4_attn.cu: shared-memory limits, scratch
-int sample_init(mlm_ctx *ctx);    // sample.cu: shared-memory and cluster limits
+int sample_init(mlm_ctx *ctx);    // sample.cu: the shared-memory limit
+// a token per row; with `step`, row r's number is uniform[*step * rows + r] (a captured
+// decode step replayed over a list of numbers)
+int sample_launch(mlm_ctx *ctx, const float *logits, int rows, int n, int64_t row_stride,
+                  const mlm_sample_params *params, const float *uniform, const int32_t *step,
+                  int32_t *token, float *prob, cudaStream_t stream);
+int sample_max_n();
 // kv4.cu: the checks every call on a 4-bit cache makes of it
 int kv4_check(mlm_ctx *ctx, const mlm_kv4_cache *cache, const char *what);
 int q6k_init(mlm_ctx *ctx);  // q6k.cu: the GEMV's shared-memory limit

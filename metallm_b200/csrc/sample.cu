@@ -547,7 +547,8 @@ struct Row {
 
 __global__ void __launch_bounds__(kThreads, 1) sample_kernel(
     const float *logits, int n, long long row_stride, int slice, int resident, int mass_bits,
-    const mlm_sample_params *params, const float *uniform, int32_t *token, float *prob) {
+    const mlm_sample_params *params, const float *uniform, const int32_t *step, int32_t *token,
+    float *prob) {
   extern __shared__ __align__(16) uint8_t s_raw[];
   Shared &s = *reinterpret_cast<Shared *>(s_raw);
   float *s_x = reinterpret_cast<float *>(s_raw + sizeof(Shared));
@@ -643,7 +644,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(
   Weights W;
   W.set(top, p.temperature, mass_bits, s.exp2_256);
   const double min_w = p.min_p > 0.f ? fmin((double)p.min_p, 1.0) : 0.0;
-  float u = uniform[row];
+  // step: rows of uniforms per step of a replayed graph
+  float u = uniform[(step ? (size_t)*step * (gridDim.x / ctas) : 0) + row];
   u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;  // NaN: 0
   u64 cut = kAll;
   bool listed = is_short && sent <= kCand;
@@ -739,6 +741,40 @@ int sample_init(mlm_ctx *ctx) {
   return MLM_OK;
 }
 
+int sample_launch(mlm_ctx *ctx, const float *logits, int rows, int n, int64_t row_stride,
+                  const mlm_sample_params *params, const float *uniform, const int32_t *step,
+                  int32_t *token, float *prob, cudaStream_t stream) {
+  int ctas = kMaxCluster;
+  // twice the SMs' number of CTAs: rows of different settings take different times
+  while (ctas > 1 && (rows * ctas > 2 * ctx->sm_count || n < kMinSlice * ctas)) ctas /= 2;
+  const int slice = (n + ctas - 1) / ctas;
+  const int resident = (size_t)slice * 4 <= kSliceBytes;
+  int bits = 62;
+  while ((1ll << (62 - bits)) < n) --bits;
+  bits = std::min(bits, 50);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Shared) + (resident ? (size_t)slice * 4 : 0);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return check_launch_pdl(ctx,
+                          cudaLaunchKernelEx(&cfg, sample_kernel, logits, n, (long long)row_stride,
+                                             slice, resident, bits, params, uniform, step, token,
+                                             prob),
+                          "mlm_sample_f32");
+}
+
+int sample_max_n() { return kMaxN; }
+
 }  // namespace mlm
 
 using namespace mlm;
@@ -756,30 +792,6 @@ extern "C" int mlm_sample_f32(mlm_ctx *ctx, const float *logits, int rows, int n
                        aligned4(prob),
               MLM_ERR_ALIGN, "mlm_sample_f32: buffers must be 4-byte aligned");
   DeviceGuard guard(ctx);
-  int ctas = kMaxCluster;
-  // twice the SMs' number of CTAs: rows of different settings take different times
-  while (ctas > 1 && (rows * ctas > 2 * ctx->sm_count || n < kMinSlice * ctas)) ctas /= 2;
-  const int slice = (n + ctas - 1) / ctas;
-  const int resident = (size_t)slice * 4 <= kSliceBytes;
-  int bits = 62;
-  while ((1ll << (62 - bits)) < n) --bits;
-  bits = std::min(bits, 50);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * ctas));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Shared) + (resident ? (size_t)slice * 4 : 0);
-  cfg.stream = ctx->stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ctas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return check_launch_pdl(ctx,
-                          cudaLaunchKernelEx(&cfg, sample_kernel, logits, n, (long long)row_stride,
-                                             slice, resident, bits, params, uniform, token, prob),
-                          "mlm_sample_f32");
+  return sample_launch(ctx, logits, rows, n, row_stride, params, uniform, nullptr, token, prob,
+                       ctx->stream);
 }

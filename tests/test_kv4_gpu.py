@@ -180,7 +180,7 @@ def _attention_case(ctx, batch, tokens, n_heads, n_kv, lens, counts, out_type, c
     return got
 
 
-@pytest.mark.parametrize("n_heads,n_kv", [(32, 8), (64, 8), (8, 8), (3, 1), (16, 1), (40, 8), (14, 2), (24, 1)])
+@pytest.mark.parametrize("n_heads,n_kv", [(32, 8), (64, 8), (8, 8), (3, 1), (16, 1), (40, 8), (14, 2), (20, 1)])
 @pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 31, 33, 64, 100, 255, 1025])
 def test_decode_lengths(ctx, n_heads, n_kv, length):
     _attention_case(ctx, 1, 1, n_heads, n_kv, [length], None, TYPE_F16, capacity=length + 5)
