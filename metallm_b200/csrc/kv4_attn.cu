@@ -51,6 +51,11 @@ constexpr int kHalfStage = kBlk * kRow;      // K or V of a block
 constexpr int kStage = 2 * kHalfStage;
 constexpr int kPieceRow = kD + 4;            // a column of a piece: o[128], m, l, padding
 constexpr int kMaxCols = 16;
+// Weights are 2^(s - max + bias), a score at most 2^kLead above the maximum, and p d has
+// to be an fp16 value: with V's scales below 2 up to 2^15, else (d < 2^13.1, the largest
+// that the append writes) up to 2^14.1.  A weight 2^24 times smaller than the largest still
+// keeps the bits of its hi part and lo part that a long cache's sum needs.
+constexpr float kLead = 4.f, kBias = 10.f, kBiasWide = -3.f;
 
 // a product from zero accumulators
 __device__ __forceinline__ void mma_f16_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -117,6 +122,34 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b),
                             *reinterpret_cast<const __half2 *>(&c));
   return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+// The four nibbles of each 16-bit half as subnormal binary16 values, a power of two each
+// (code_unit) times the code.  A product's terms are aligned by their operands' exponents,
+// which are all that of the largest subnormal, and cut off below some 2^-24 of the largest
+// term's: a code k bits below the top loses k bits, always downwards, and a sum over a long
+// cache nearly cancels with its m part.  In place (bits 0 and 4) that cost an fp16 output of
+// 60001 rows 5e-4 of its norm, against 2.1e-4 for its rounding.  So all four come to bit 4
+// for it (three shifts, 64 x 8192 rows 120.8 us); for a bf16 output, whose rounding is eight
+// times coarser, one shift takes two of them to bits 2 and 6 (115.8 us, 112.8 in place).
+template <bool EXACT>
+__device__ __forceinline__ void spread_codes(uint32_t w, uint32_t (&v)[4]) {
+  if (EXACT) {
+    v[0] = (w << 4) & 0x00F000F0u;
+    v[1] = w & 0x00F000F0u;
+    v[2] = (w >> 4) & 0x00F000F0u;
+    v[3] = (w >> 8) & 0x00F000F0u;
+  } else {
+    v[0] = (w << 2) & 0x003C003Cu;
+    v[1] = (w << 2) & 0x03C003C0u;
+    v[2] = (w >> 6) & 0x003C003Cu;
+    v[3] = (w >> 6) & 0x03C003C0u;
+  }
+}
+// 2^24 over the factor of nibble i
+template <bool EXACT>
+__device__ __forceinline__ float code_unit(int i) {
+  return EXACT ? 1048576.f : (i & 1) ? 262144.f : 4194304.f;
 }
 
 // an item (the blocks of one KV head of one sequence) and a block of it
@@ -355,6 +388,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
   int seen[NT];                // rows column r attends to
   uint32_t qm[NT][2];          // the B operand of K's minima: (0, group sum) per group, hi and lo
   float o[NT][4][2][4], mx[NT], l[NT];
+  float bias = kBias;          // of the weights' exponent: kBiasWide once a V scale is 2 or more
   float om[NT][4];             // sum of p m: rows 2 g + 1 of the product with V's scales
   bool ok = true;
   int stage = 0;
@@ -369,6 +403,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
       const Item cur = s_cur[warp];
       const int len = cur.len, count = cur.count;
       mask_from = max(0, len - count + 1) / kBlk;
+      bias = kBias;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int col = DUP ? (r & 3) : nt * 8 + r;
@@ -505,15 +540,42 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
         const uint32_t bits = good >> (4 * kt + 2 * j);
         return ((bits & 1) ? 0xFFFFu : 0u) | ((bits & 2) ? 0xFFFF0000u : 0u);
       };
+      // V's transposed scale words: d in the lanes of even r, m in the others.  A scale of
+      // 2 or more has bit 14 set
+      uint32_t mt[2][2];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        ldsm2_t(sv + (kt * 16 + (lane & 15)) * kRow + 64, mt[kt]);
+        if (MASK) {
+          mt[kt][0] &= good_pair(kt, 0);
+          mt[kt][1] &= good_pair(kt, 1);
+        }
+      }
+      {
+        const uint32_t bits = (mt[0][0] | mt[0][1] | mt[1][0] | mt[1][1]) & (r & 1 ? 0u : 0x40004000u);
+        if (__any_sync(0xffffffffu, bits != 0) && bias == kBias) {
+          const float f = 1.f / (1 << (int)(kBias - kBiasWide));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            l[nt] *= f;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              om[nt][g] *= f;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[nt][g][0][i] *= f, o[nt][g][1][i] *= f;
+            }
+          }
+          bias = kBiasWide;
+        }
+      }
       // Running maximum and sum.  The maximum follows only when a score leads it
-      // by more than 2^8: the weights are 2^(s - max - 6), so at most 4, and p d stays
-      // an fp16 value for every d below 2^14; the factor is l's too.
+      // by more than 2^kLead; the factor is l's too.
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, sT[nt][i >> 2][(i >> 1) & 1][i & 1]);
-        if (__any_sync(0xffffffffu, (top - mx[nt]) * cs[nt] > 8.f)) {
+        if (__any_sync(0xffffffffu, (top - mx[nt]) * cs[nt] > kLead)) {
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           top = fmaxf(top, mx[nt]);
@@ -534,7 +596,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
           }
           mx[nt] = top;
         }
-        const float base = fmaf(mx[nt] == -INFINITY ? 0.f : mx[nt], -cs[nt], -6.f);
+        const float base = fmaf(mx[nt] == -INFINITY ? 0.f : mx[nt], -cs[nt], bias);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float &v = sT[nt][i >> 2][(i >> 1) & 1][i & 1];
@@ -570,24 +632,20 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
               }
             }
           }
-        // sum_j p_j m_jg (and p_j d_jg, unused): the transposed scale words
-        uint32_t mt[2];
-        ldsm2_t(sv + (kt * 16 + (lane & 15)) * kRow + 64, mt);
-        if (MASK) {
-          mt[0] &= good_pair(kt, 0);
-          mt[1] &= good_pair(kt, 1);
-        }
+        // sum_j p_j m_jg (and p_j d_jg, unused)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const uint32_t b0 = kSplit && lo_lane ? pl[nt][0] : ph[nt][0],
                          b1 = kSplit && lo_lane ? pl[nt][1] : ph[nt][1];
-          mma_f16_16816(om[nt], mt[0], 0u, mt[1], 0u, b0, b1);
-          if (LO && !DUP) mma_f16_16816(om[nt], mt[0], 0u, mt[1], 0u, pl[nt][0], pl[nt][1]);
+          mma_f16_16816(om[nt], mt[kt][0], 0u, mt[kt][1], 0u, b0, b1);
+          if (LO && !DUP) mma_f16_16816(om[nt], mt[kt][0], 0u, mt[kt][1], 0u, pl[nt][0], pl[nt][1]);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const uint32_t wa = w[g >> 1][(g & 1) * 2], wb = w[g >> 1][(g & 1) * 2 + 1];
-          const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
+          uint32_t va[4], vb[4];
+          spread_codes<LO>(wa, va);
+          spread_codes<LO>(wb, vb);
           // d of rows 2 t4, + 1 and of rows 2 t4 + 8, + 9
           uint32_t dd[2] = {__byte_perm(u4_get(dm[0], g), u4_get(dm[1], g), 0x5410),
                             __byte_perm(u4_get(dm[2], g), u4_get(dm[3], g), 0x5410)};
@@ -612,15 +670,11 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
               }
             }
             const uint32_t b0 = bh[0], b1 = bh[1], l0 = bl[0], l1 = bl[1];
-            mma_f16_16816(o[nt][g][0], wa & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x000F000Fu,
-                          wb & 0x00F000F0u, b0, b1);
-            mma_f16_16816(o[nt][g][1], wa8 & 0x000F000Fu, wa8 & 0x00F000F0u, wb8 & 0x000F000Fu,
-                          wb8 & 0x00F000F0u, b0, b1);
+            mma_f16_16816(o[nt][g][0], va[0], va[1], vb[0], vb[1], b0, b1);
+            mma_f16_16816(o[nt][g][1], va[2], va[3], vb[2], vb[3], b0, b1);
             if (LO && !DUP) {
-              mma_f16_16816(o[nt][g][0], wa & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x000F000Fu,
-                            wb & 0x00F000F0u, l0, l1);
-              mma_f16_16816(o[nt][g][1], wa8 & 0x000F000Fu, wa8 & 0x00F000F0u,
-                            wb8 & 0x000F000Fu, wb8 & 0x00F000F0u, l0, l1);
+              mma_f16_16816(o[nt][g][0], va[0], va[1], vb[0], vb[1], l0, l1);
+              mma_f16_16816(o[nt][g][1], va[2], va[3], vb[2], vb[3], l0, l1);
             }
           }
         }
@@ -672,8 +726,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
             for (int c = 0; c < 4; ++c) {
               float w = o[nt][g][i][c];
               if (kSplit) w += __shfl_xor_sync(0xffffffffu, w, 2);  // hi + lo
-              // the codes' unit: 2^-24, and 16 times that in rows 8 .. 15
-              v[c & 1][2 * i + (c >> 1)] = fmaf(w, c < 2 ? 16777216.f : 1048576.f, (c & 1) ? m1 : m0);
+              v[c & 1][2 * i + (c >> 1)] = fmaf(w, code_unit<LO>(c >> 1), (c & 1) ? m1 : m0);
             }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -699,7 +752,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
           }
         }
         if (!whole && t4 == 0 && (!DUP || r < 4)) {
-          piece[(nt * 8 + r) * kPieceRow + kD] = mx[nt] * cs[nt];
+          piece[(nt * 8 + r) * kPieceRow + kD] = fmaf(mx[nt], cs[nt], -bias);
           piece[(nt * 8 + r) * kPieceRow + kD + 1] = l[nt];
         }
       }

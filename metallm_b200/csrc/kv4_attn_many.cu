@@ -13,9 +13,10 @@
 //   - 4 warps per row tile do the softmax, a thread per row: S from TMEM, the
 //     weights back as fp16 over it, where the second product reads them as its A
 //     operand.
-// The running maximum follows only when a score leads it by more than 2^14 (a
-// weight is then still an fp16 value of full precision), so the accumulator in
-// TMEM is rescaled once in a row's life, as a rule.  Scores, maxima and sums are
+// The running maximum follows only when a score leads it by more than 2^12, so the
+// accumulator in TMEM is rescaled once in a row's life, as a rule.  The weights are
+// 2^(s - max + 3): at most 2^15, and fp16 values of full precision down to 2^-17 of the
+// maximum's, as the many small ones of a long cache want.  Scores, maxima and sums are
 // fp32; K, V and the weights are fp16 operands.
 //
 // V^T is the N-major B operand of the second product: both K and V lie in
@@ -63,7 +64,7 @@ constexpr size_t smem_bytes(int batch) { return kOffLine + 8 * (size_t)(batch + 
 constexpr int kTmemCols = 512;  // S/P of tile 0 and 1, O of tile 0 and 1
 constexpr int kPartFloats = kRows * (kKv4D + 2);  // o, then m and l
 constexpr float kScale2 = kInvSqrtD * kLog2e;
-constexpr float kLead = 14.f / kScale2;
+constexpr float kBias = 3.f, kLead = 12.f / kScale2;
 
 // instruction descriptors: fp16 A and B, fp32 accumulators, M = N = 128; B K-major
 // (S = Q K^T) or N-major (O = P V)
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
         auto weights = [&](auto mask_tag) {
           constexpr bool MASK = decltype(mask_tag)::value;
           uint32_t s[2][32];
-          float m2 = m == -INFINITY ? 0.f : -m * kScale2;
+          float m2 = m == -INFINITY ? 0.f : fmaf(-m, kScale2, kBias);
           tmem_ld32(ts, s[0]);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -458,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
               const float2 l = unpair(l2);
               l2 = pair(l.x * f, l.y * f);
               m = up;
-              m2 = m == -INFINITY ? 0.f : -m * kScale2;
+              m2 = m == -INFINITY ? 0.f : fmaf(-m, kScale2, kBias);
             }
             const uint64_t mm = pair(m2, m2), cc = pair(kScale2, kScale2);
             uint32_t w[16];

@@ -133,15 +133,17 @@ def test_append_outside_the_cache_is_skipped_and_reported(ctx, pos, counts):
 
 
 def _attention_case(ctx, batch, tokens, n_heads, n_kv, lens, counts, out_type, capacity=None, seed=0,
-                    spoil=True, q_scale=1.5):
+                    spoil=True, q_scale=1.5, v_scale=None):
     """Runs mlm_attn_kv4 and compares it with the 64-bit form.  `spoil`: rows past a sequence's
-    length hold NaN scales."""
+    length hold NaN scales.  `v_scale`: factors of V per position."""
     rng = np.random.default_rng(seed + 1000 * tokens + batch)
     capacity = capacity or max(max(lens), 1)
     rows = []
-    for _ in "kv":
+    for name in "kv":
         x = rng.standard_normal((batch, n_kv, capacity, R.D)).astype(np.float32)
         x[..., 5::61] *= 4
+        if name == "v" and v_scale is not None:
+            x *= v_scale(np.arange(capacity, dtype=np.float32))[:, None]
         r = R.quantize(x)
         if spoil:
             for b in range(batch):
@@ -184,6 +186,16 @@ def _attention_case(ctx, batch, tokens, n_heads, n_kv, lens, counts, out_type, c
 @pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 31, 33, 64, 100, 255, 1025])
 def test_decode_lengths(ctx, n_heads, n_kv, length):
     _attention_case(ctx, 1, 1, n_heads, n_kv, [length], None, TYPE_F16, capacity=length + 5)
+
+
+@pytest.mark.parametrize("tokens,n_heads", [(1, 4), (1, 12), (5, 4)])
+@pytest.mark.parametrize("v_scale", ["one", "small", "large", "mixed"])
+def test_long_cache_keeps_the_small_weights(ctx, tokens, n_heads, v_scale):
+    """Many rows of little weight each, whose sum nearly cancels: the weights need more bits than the
+    largest one's fp16 step, whatever V's scale, and where V grows on the way."""
+    scale = {"one": lambda j: 1 + 0 * j, "small": lambda j: 0.02 + 0 * j, "large": lambda j: 3000 + 0 * j,
+             "mixed": lambda j: np.where(j % 997 == 500, 40, 1).astype(np.float32)}[v_scale]
+    _attention_case(ctx, 1, tokens, n_heads, 1, [60001], None, TYPE_F16, capacity=60010, v_scale=scale)
 
 
 @pytest.mark.parametrize("out_type", [TYPE_F16, TYPE_BF16])
