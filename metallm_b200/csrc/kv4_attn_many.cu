@@ -17,7 +17,9 @@
 // accumulator in TMEM is rescaled once in a row's life, as a rule.  The weights are
 // 2^(s - max + 3): at most 2^15, and fp16 values of full precision down to 2^-17 of the
 // maximum's, as the many small ones of a long cache want.  Scores, maxima and sums are
-// fp32; K, V and the weights are fp16 operands.
+// fp32.  For a bf16 output K, V and the weights are fp16 operands, each rounded once; an
+// fp16 output, eight times finer, would show that (up to three times its own rounding),
+// so there each is hi + lo: two products for the scores, three for O.
 //
 // V^T is the N-major B operand of the second product: both K and V lie in
 // shared memory as [key][dimension] in the 128-byte swizzle, the eight
@@ -192,6 +194,13 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// x and y as fp16 pairs hi + lo
+__device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32_t &lo) {
+  hi = pack_f16(x, y);
+  const float2 h = unpack_f16(hi);
+  lo = pack_f16(x - h.x, y - h.y);
+}
+
 __device__ __forceinline__ int row_tiles(int count, int group) {
   return (count * group + kRows - 1) / kRows;
 }
@@ -257,26 +266,37 @@ struct Walk {
   }
 };
 
-// one word of codes to eight fp16 values in the order 0 4 1 5 2 6 3 7
-__device__ __forceinline__ uint4 values8(uint32_t w, __half2 d, __half2 m) {
+// one word of codes to eight fp16 values in the order 0 4 1 5 2 6 3 7, and with LO
+// what rounding left of them, as fp16
+template <bool LO>
+__device__ __forceinline__ void values8(uint32_t w, __half2 d, __half2 m, uint4 &value, uint4 &rest) {
   // codes in the mantissa of 1024 (of 64 where they sit 4 bits higher)
   const __half2 one = __float2half2_rn(-1024.f), low = __float2half2_rn(-64.f),
                 sixteenth = __float2half2_rn(0.0625f);
-  uint32_t v[4];
+  const uint64_t df = pair(__low2float(d), __low2float(d)), mf = pair(__low2float(m), __low2float(m));
+  uint32_t v[4], e[4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t x = i ? w >> 8 : w;
-    const uint32_t a = (x & 0x000F000Fu) | 0x64006400u, b = (x & 0x00F000F0u) | 0x64006400u;
-    const __half2 ca = __hadd2(*reinterpret_cast<const __half2 *>(&a), one);
-    const __half2 cb = __hfma2(*reinterpret_cast<const __half2 *>(&b), sixteenth, low);
-    const __half2 va = __hfma2(ca, d, m), vb = __hfma2(cb, d, m);
-    v[2 * i] = *reinterpret_cast<const uint32_t *>(&va);
-    v[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&vb);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = i < 2 ? w : w >> 8;
+    const uint32_t a = (x & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;
+    const __half2 ha = *reinterpret_cast<const __half2 *>(&a);
+    const __half2 c = i & 1 ? __hfma2(ha, sixteenth, low) : __hadd2(ha, one);
+    const __half2 h = __hfma2(c, d, m);
+    v[i] = *reinterpret_cast<const uint32_t *>(&h);
+    if (LO) {
+      const float2 cf = __half22float2(c), hf = __half22float2(h);
+      const float2 r = unpair(add2(fma2(pair(cf.x, cf.y), df, mf), pair(-hf.x, -hf.y)));
+      e[i] = pack_f16(r.x, r.y);
+    }
   }
-  return make_uint4(v[0], v[1], v[2], v[3]);
+  value = make_uint4(v[0], v[1], v[2], v[3]);
+  if (LO) rest = make_uint4(e[0], e[1], e[2], e[3]);
 }
 template <class OutT>
 __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs a) {
+  // hi + lo operands, each in one buffer of the two instead of one in two
+  constexpr bool EXACT = std::is_same<OutT, __half>::value;
+  constexpr uint32_t kStages = EXACT ? 1 : 2;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = (uint32_t)__cvta_generic_to_shared(smem);
   const uint32_t bar = sbase + kOffBar;
@@ -439,20 +459,35 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
                 }
               }
               tmem_wait_st();
+              if (EXACT) {
 #pragma unroll 1
-              for (int j = 0; j < (c + 1) / 2; ++j) {  // 64 weights at a time
-                uint32_t o[32];
-                tmem_ld32(ts + 32 * j, o);
-                tmem_wait_ld(o);
-                uint32_t h[16];
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
+                for (int j = 0; j < c; ++j) {
+                  uint32_t o[32];
+                  tmem_ld32(ts + 32 * j, o);
+                  tmem_wait_ld(o);
 #pragma unroll
                   for (int k = 0; k < 16; ++k) {
-                    const float2 e = unpack_f16(o[16 * half + k]);
-                    h[k] = pack_f16(e.x * f, e.y * f);
+                    const float2 h = unpack_f16(o[k]), e = unpack_f16(o[16 + k]);
+                    split_f16((h.x + e.x) * f, (h.y + e.y) * f, o[k], o[16 + k]);
                   }
-                  if (2 * j + half < c) tmem_st16(ts + 32 * j + 16 * half, h);
+                  tmem_st32(ts + 32 * j, o);
+                }
+              } else {
+#pragma unroll 1
+                for (int j = 0; j < (c + 1) / 2; ++j) {  // 64 weights at a time
+                  uint32_t o[32];
+                  tmem_ld32(ts + 32 * j, o);
+                  tmem_wait_ld(o);
+                  uint32_t h[16];
+#pragma unroll
+                  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                      const float2 e = unpack_f16(o[16 * half + k]);
+                      h[k] = pack_f16(e.x * f, e.y * f);
+                    }
+                    if (2 * j + half < c) tmem_st16(ts + 32 * j + 16 * half, h);
+                  }
                 }
               }
               tmem_wait_st();
@@ -462,16 +497,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
               m2 = m == -INFINITY ? 0.f : fmaf(-m, kScale2, kBias);
             }
             const uint64_t mm = pair(m2, m2), cc = pair(kScale2, kScale2);
-            uint32_t w[16];
+            uint32_t w[16], rest[16];
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
               const float2 e =
                   unpair(fma2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), cc, mm));
               const float p0 = ex2(e.x), p1 = ex2(e.y);
               l2 = add2(l2, pair(p0, p1));
-              w[k / 2] = pack_f16(p0, p1);
+              if (EXACT)
+                split_f16(p0, p1, w[k / 2], rest[k / 2]);
+              else
+                w[k / 2] = pack_f16(p0, p1);
             }
-            tmem_st16(ts + 16 * c, w);  // over scores that have been read
+            // over scores that have been read
+            tmem_st16(ts + (EXACT ? 32 : 16) * c, w);
+            if (EXACT) tmem_st16(ts + 32 * c + 16, rest);
           }
         };
         if (__any_sync(0xffffffffu, lim < kTile))
@@ -560,10 +600,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
     int kt = walk.p.kt0;
     if (more) load(walk.p, kt);
     while (more) {
-      const uint32_t buf = n_kv & 1;
-      if (n_kv >= 2) {
+      const uint32_t buf = n_kv % kStages;
+      if (n_kv >= kStages) {
         ok = __all_sync(0xffffffffu,
-                        mbar_wait_bounded(empty + 8 * buf, ((n_kv >> 1) - 1) & 1, a.status));
+                        mbar_wait_bounded(empty + 8 * buf, (n_kv / kStages - 1) & 1, a.status));
         if (!ok) break;
       }
       uint4 cur[5];
@@ -587,8 +627,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
         const __half2 d = *reinterpret_cast<const __half2 *>(&dd),
                       m = *reinterpret_cast<const __half2 *>(&mm);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint4 *>(dst + chunk_at(key, 4 * g + i)) = values8(u4_get(cur[g], i), d, m);
+        for (int i = 0; i < 4; ++i) {
+          uint4 value, rest;
+          values8<EXACT>(u4_get(cur[g], i), d, m, value, rest);
+          *reinterpret_cast<uint4 *>(dst + chunk_at(key, 4 * g + i)) = value;
+          if (EXACT) *reinterpret_cast<uint4 *>(dst + 2 * kOperand + chunk_at(key, 4 * g + i)) = rest;
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -607,15 +651,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
       const uint32_t d = tmem + tile * kTile;
       mma_smem<false>(d, q, kb);
 #pragma unroll
-      for (int k = 1; k < 8; ++k) {
-        constexpr int kStep = 32 >> 4, kHalf = kSub >> 4;
-        mma_smem<true>(d, q + (k >> 2) * kHalf + (k & 3) * kStep,
-                       kb + (k >> 2) * kHalf + (k & 3) * kStep);
+      for (int k = 1; k < (EXACT ? 16 : 8); ++k) {
+        constexpr int kStep = 32 >> 4, kHalf = kSub >> 4, kLo = 2 * kOperand >> 4;
+        mma_smem<true>(d, q + ((k >> 2) & 1) * kHalf + (k & 3) * kStep,
+                       kb + (k >> 3) * kLo + ((k >> 2) & 1) * kHalf + (k & 3) * kStep);
       }
       commit(bar + 8 * (kSfull + tile));
     };
     auto ready = [&](int which, uint32_t n) {
-      const bool in_time = mbar_wait_bounded(bar + 8 * (which + (n & 1)), (n >> 1) & 1, a.status);
+      const bool in_time = mbar_wait_bounded(bar + 8 * (which + n % kStages), (n / kStages) & 1, a.status);
       tc_fence_after();
       return in_time;
     };
@@ -625,10 +669,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
       ok = mbar_wait_bounded(bar + 8 * kQfull, n_item & 1, a.status) && ready(kKfull, n_kv);
       if (!ok) break;
       ++n_item;
-      for (int i = 0; i < tiles; ++i) scores(i, n_kv & 1);
-      commit(bar + 8 * (kKempty + (n_kv & 1)));
+      for (int i = 0; i < tiles; ++i) scores(i, n_kv % kStages);
+      commit(bar + 8 * (kKempty + n_kv % kStages));
       for (int kt = p.kt0; ok && kt < p.kt1; ++kt, ++n_kv) {
-        const uint32_t vb = v0 + (n_kv & 1) * (2 * kOperand >> 4);
+        const uint32_t vb = v0 + (n_kv % kStages) * (2 * kOperand >> 4);
         for (int i = 0; i < tiles; ++i) {
           ok = (i > 0 || ready(kVfull, n_kv)) &&
                mbar_wait_bounded(bar + 8 * (kPfull + i), n_p[i] & 1, a.status);
@@ -636,15 +680,26 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
           ++n_p[i];
           tc_fence_after();
           mma_tmem(tmem + (2 + i) * kTile, tmem + i * kTile, vb, kt > p.kt0);
+          if (EXACT) {  // 32 weights' hi, then their lo
 #pragma unroll
-          for (int k = 1; k < 8; ++k)
-            mma_tmem(tmem + (2 + i) * kTile, tmem + i * kTile + 8 * k, vb + k * (2048 >> 4), 1);
-          if (i == tiles - 1) commit(bar + 8 * (kVempty + (n_kv & 1)));
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t d = tmem + (2 + i) * kTile, w = tmem + i * kTile + 32 * (k >> 1) + 8 * (k & 1);
+              const uint32_t v = vb + k * (2048 >> 4);
+              if (k > 0) mma_tmem(d, w, v, 1);
+              mma_tmem(d, w + 16, v, 1);
+              mma_tmem(d, w, v + (2 * kOperand >> 4), 1);
+            }
+          } else {
+#pragma unroll
+            for (int k = 1; k < 8; ++k)
+              mma_tmem(tmem + (2 + i) * kTile, tmem + i * kTile + 8 * k, vb + k * (2048 >> 4), 1);
+          }
+          if (i == tiles - 1) commit(bar + 8 * (kVempty + n_kv % kStages));
           if (kt + 1 < p.kt1) {
             ok = i > 0 || ready(kKfull, n_kv + 1);
             if (!ok) break;
-            scores(i, (n_kv + 1) & 1);
-            if (i == tiles - 1) commit(bar + 8 * (kKempty + ((n_kv + 1) & 1)));
+            scores(i, (n_kv + 1) % kStages);
+            if (i == tiles - 1) commit(bar + 8 * (kKempty + (n_kv + 1) % kStages));
           } else {
             commit(bar + 8 * (kOfull + i));
           }

@@ -168,7 +168,7 @@ def _attention_case(ctx, batch, tokens, n_heads, n_kv, lens, counts, out_type, c
     assert np.all(got[~live] == 77)  # rows behind the last token are left as they were
     assert np.all(np.isfinite(got[live]))
     eps = 2.0 ** -10 if out_type == TYPE_F16 else 2.0 ** -7
-    rounded = tokens * (n_heads // n_kv) > 16
+    rounded = tokens * (n_heads // n_kv) > 16 and out_type != TYPE_F16
     tol = R.attention_tolerance(ref, smax, vmax, eps, rounded)
     bad = np.abs(got - ref) > tol
     assert not np.any(bad[live]), (np.argwhere(bad & live[..., None])[:5], np.abs(got - ref)[live].max())
@@ -188,7 +188,7 @@ def test_decode_lengths(ctx, n_heads, n_kv, length):
     _attention_case(ctx, 1, 1, n_heads, n_kv, [length], None, TYPE_F16, capacity=length + 5)
 
 
-@pytest.mark.parametrize("tokens,n_heads", [(1, 4), (1, 12), (5, 4)])
+@pytest.mark.parametrize("tokens,n_heads", [(1, 4), (1, 12), (5, 4), (9, 4)])
 @pytest.mark.parametrize("v_scale", ["one", "small", "large", "mixed"])
 def test_long_cache_keeps_the_small_weights(ctx, tokens, n_heads, v_scale):
     """Many rows of little weight each, whose sum nearly cancels: the weights need more bits than the
