@@ -67,6 +67,19 @@ __device__ __forceinline__ void mma_f16_zero(float (&c)[4], uint32_t a0, uint32_
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
+// a += b.  A product's accumulators are cut off, not rounded: left in them over a long
+// stretch the codes' and the minima's parts of an output, which nearly cancel, shrink by
+// some 2^-24 of themselves per product (16 sequences of 131072 rows: an error of 4.5e-3 of
+// the norm, 1.7e-3 with a block's products from zero and added here).
+__device__ __forceinline__ void add4(float (&a)[4], const float (&b)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i += 2)
+    asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n"
+        " add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+        : "+f"(a[i]), "+f"(a[i + 1])
+        : "f"(b[i]), "f"(b[i + 1]));
+}
+
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -604,79 +617,92 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
           l[nt] += v;
         }
       }
-      // o += (p d) c and the m part
+      // the weights of the lane's eight rows as fp16 hi (and lo) pairs, and the m part:
+      // sum_j p_j m_jg (and p_j d_jg, unused)
+      uint32_t ph[NT][2][2], pl[NT][2][2], pn[NT][2][2];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        uint32_t w[2][4];
-        ldsm4_t(sv + kt * 16 * kRow + tile_lane, w[0]);
-        ldsm4_t(sv + kt * 16 * kRow + tile_lane + 32, w[1]);
-        uint4 dm[4];
+      for (int nt = 0; nt < NT; ++nt) {
+        float sum[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          dm[i] = lds16(sv + (kt * 16 + (i >> 1) * 8 + 2 * t4 + (i & 1)) * kRow + 64);
-        // the weights of the lane's four rows as fp16 hi (and lo) pairs
-        uint32_t ph[NT][2], pl[NT][2], pn[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float(&p)[2] = sT[nt][kt][j];
-            ph[nt][j] = pack_f16(p[0], p[1]);
-            pl[nt][j] = pn[nt][j] = 0;
+            uint32_t &h = ph[nt][kt][j], &lo = pl[nt][kt][j], &n = pn[nt][kt][j];
+            h = pack_f16(p[0], p[1]);
+            lo = n = 0;
             if (LO) {
-              const float2 h = unpack_f16(ph[nt][j]);
-              pl[nt][j] = pack_f16(p[0] - h.x, p[1] - h.y);
+              const float2 f = unpack_f16(h);
+              lo = pack_f16(p[0] - f.x, p[1] - f.y);
               if (DUP) {
-                pl[nt][j] = lo_lane ? pl[nt][j] : 0u;
-                pn[nt][j] = lo_lane ? ph[nt][j] ^ 0x80008000u : 0u;
+                lo = lo_lane ? lo : 0u;
+                n = lo_lane ? h ^ 0x80008000u : 0u;
               }
             }
           }
-        // sum_j p_j m_jg (and p_j d_jg, unused)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const uint32_t b0 = kSplit && lo_lane ? pl[nt][0] : ph[nt][0],
-                         b1 = kSplit && lo_lane ? pl[nt][1] : ph[nt][1];
-          mma_f16_16816(om[nt], mt[kt][0], 0u, mt[kt][1], 0u, b0, b1);
-          if (LO && !DUP) mma_f16_16816(om[nt], mt[kt][0], 0u, mt[kt][1], 0u, pl[nt][0], pl[nt][1]);
+          const uint32_t b0 = kSplit && lo_lane ? pl[nt][kt][0] : ph[nt][kt][0],
+                         b1 = kSplit && lo_lane ? pl[nt][kt][1] : ph[nt][kt][1];
+          if (kt == 0)
+            mma_f16_zero(sum, mt[kt][0], 0u, mt[kt][1], 0u, b0, b1);
+          else
+            mma_f16_16816(sum, mt[kt][0], 0u, mt[kt][1], 0u, b0, b1);
+          if (LO && !DUP) mma_f16_16816(sum, mt[kt][0], 0u, mt[kt][1], 0u, pl[nt][kt][0], pl[nt][kt][1]);
         }
+        add4(om[nt], sum);
+      }
+      // o += (p d) c
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const uint32_t wa = w[g >> 1][(g & 1) * 2], wb = w[g >> 1][(g & 1) * 2 + 1];
-          uint32_t va[4], vb[4];
-          spread_codes<LO>(wa, va);
-          spread_codes<LO>(wb, vb);
-          // d of rows 2 t4, + 1 and of rows 2 t4 + 8, + 9
-          uint32_t dd[2] = {__byte_perm(u4_get(dm[0], g), u4_get(dm[1], g), 0x5410),
-                            __byte_perm(u4_get(dm[2], g), u4_get(dm[3], g), 0x5410)};
-          if (MASK) {
-            dd[0] &= good_pair(kt, 0);
-            dd[1] &= good_pair(kt, 1);
-          }
+      for (int gp = 0; gp < 2; ++gp) {
+        uint32_t w[2][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            uint32_t bh[2], bl[2] = {0, 0};
+        for (int kt = 0; kt < 2; ++kt) ldsm4_t(sv + kt * 16 * kRow + tile_lane + 32 * gp, w[kt]);
+#pragma unroll
+        for (int gi = 0; gi < 2; ++gi) {
+          const int g = 2 * gp + gi;
+          uint32_t bh[NT][2][2], bl[NT][2][2];
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const uint32_t d = dd[j];
-              // p d = hi + lo: hi the rounded product, lo its exact rest and p_lo d
-              if (!LO) {
-                bh[j] = hmul2(ph[nt][j], d);
-              } else if (DUP) {  // hi in lanes with pn = pl = 0, lo in the others
-                bh[j] = hfma2(pl[nt][j], d, hfma2(ph[nt][j], d, hmul2(pn[nt][j], d)));
-              } else {
-                bh[j] = hmul2(ph[nt][j], d);
-                bl[j] = hfma2(pl[nt][j], d, hfma2(ph[nt][j], d, bh[j] ^ 0x80008000u));
+              // d of rows 2 t4, + 1 (and of rows 2 t4 + 8, + 9)
+              const uint32_t d = __shfl_sync(0xffffffffu, mt[kt][j], 8 * g + t4);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                uint32_t &h = bh[nt][kt][j], &lo = bl[nt][kt][j];
+                const uint32_t p = ph[nt][kt][j], rest = pl[nt][kt][j];
+                // p d = hi + lo: hi the rounded product, lo its exact rest and p_lo d
+                if (!LO) {
+                  h = hmul2(p, d);
+                } else if (DUP) {  // hi in lanes with pn = pl = 0, lo in the others
+                  h = hfma2(rest, d, hfma2(p, d, hmul2(pn[nt][kt][j], d)));
+                } else {
+                  h = hmul2(p, d);
+                  lo = hfma2(rest, d, hfma2(p, d, h ^ 0x80008000u));
+                }
               }
             }
-            const uint32_t b0 = bh[0], b1 = bh[1], l0 = bl[0], l1 = bl[1];
-            mma_f16_16816(o[nt][g][0], va[0], va[1], vb[0], vb[1], b0, b1);
-            mma_f16_16816(o[nt][g][1], va[2], va[3], vb[2], vb[3], b0, b1);
-            if (LO && !DUP) {
-              mma_f16_16816(o[nt][g][0], va[0], va[1], vb[0], vb[1], l0, l1);
-              mma_f16_16816(o[nt][g][1], va[2], va[3], vb[2], vb[3], l0, l1);
-            }
+          uint32_t va[2][4], vb[2][4];
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) {
+            spread_codes<LO>(w[kt][2 * gi], va[kt]);
+            spread_codes<LO>(w[kt][2 * gi + 1], vb[kt]);
           }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float sum[4];
+              mma_f16_zero(sum, va[0][2 * i], va[0][2 * i + 1], vb[0][2 * i], vb[0][2 * i + 1],
+                           bh[nt][0][0], bh[nt][0][1]);
+              mma_f16_16816(sum, va[1][2 * i], va[1][2 * i + 1], vb[1][2 * i], vb[1][2 * i + 1],
+                            bh[nt][1][0], bh[nt][1][1]);
+              if (LO && !DUP)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+                  mma_f16_16816(sum, va[kt][2 * i], va[kt][2 * i + 1], vb[kt][2 * i],
+                                vb[kt][2 * i + 1], bl[nt][kt][0], bl[nt][kt][1]);
+              add4(o[nt][g][i], sum);
+            }
         }
       }
     };
@@ -861,7 +887,6 @@ template <int NT, bool DUP>
 struct FewShape {
   static constexpr int warps = NT == 1 ? 16 : 8;
   static constexpr int stages = NT == 1 ? 2 : 4;
-  static constexpr int cols = DUP ? 4 : 8 * NT;
   static constexpr size_t smem(int batch) {
     return (size_t)warps * stages * kStage + sizeof(int) * (batch + 1);
   }

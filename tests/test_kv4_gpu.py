@@ -199,6 +199,32 @@ def test_long_cache_keeps_the_small_weights(ctx, tokens, n_heads, v_scale):
 
 
 @pytest.mark.parametrize("out_type", [TYPE_F16, TYPE_BF16])
+def test_many_long_caches(ctx, out_type):
+    """Long stretches of one cache in the same accumulators: 128 sequences (the same rows, their own
+    queries), the outputs' two halves (codes and minima) nearly cancelling."""
+    rng = np.random.default_rng(12)
+    batch, n_heads, n = 128, 4, 32768
+    rows = [R.quantize(rng.standard_normal((1, 1, n, R.D)).astype(np.float32)) for _ in "kv"]
+    q = (1.5 * rng.standard_normal((batch, 1, n_heads, R.D))).astype(np.float16)
+    dk, dv = (ctx.to_device(np.repeat(r, batch, axis=0)) for r in rows)
+    out = ctx.alloc(2 * q.size)
+    ctx.attn_kv4(Kv4Cache(int(dk), int(dv), batch, 1, R.D, n), ctx.to_device(q), n_heads, 1,
+                 _ints(ctx, [n] * batch), None, out, out_type)
+    ctx.wait()
+    raw = out.download(np.uint16).reshape(q.shape)
+    got = (raw.view(np.float16).astype(np.float64) if out_type == TYPE_F16
+           else (raw.astype(np.uint32) << 16).view(np.float32).astype(np.float64))
+    eps = 2.0 ** -10 if out_type == TYPE_F16 else 2.0 ** -7
+    for b in (0, 61, 127):
+        ref = R.attention(q[b:b + 1], *rows, [n], [1])[0][0]
+        # half a step of rounding, uniform: eps / 2 / sqrt(3) in the mean square; a bf16 output's
+        # weights are fp16 products p d, twice rounded (2^-11 / sqrt(3) each) against codes that are
+        # not centred (their mean square at most 2.5 of the values')
+        bound = eps / 2 / 3 ** .5 + 3e-5 + (0 if out_type == TYPE_F16 else 2.5 * 2 ** .5 * 2.0 ** -11 / 3 ** .5)
+        assert np.linalg.norm(got[b] - ref) / np.linalg.norm(ref) < bound
+
+
+@pytest.mark.parametrize("out_type", [TYPE_F16, TYPE_BF16])
 @pytest.mark.parametrize("lens", [[0], [0, 0, 0], [5, 0, 700, 1, 64, 0, 333], [2000, 1], [0, 4000],
                                   list(range(40))])
 def test_decode_ragged(ctx, lens, out_type):
