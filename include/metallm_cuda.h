@@ -425,9 +425,14 @@ int mlm_kv4_read_f16(mlm_ctx *ctx, const mlm_kv4_cache *cache, int tokens, const
  * token that attends to no row gets zeros; out rows at and past counts_dev[b]
  * are left as they were.  q fp16 and out (out_type MLM_TYPE_F16 or BF16)
  * [batch][tokens][n_heads][128], 16-byte aligned; n_heads a multiple of
- * n_kv_heads.  Scores, softmax statistics and sums are fp32.  Uses the
- * context's attention scratch: launches on one context are stream-ordered and
- * must not overlap. */
+ * n_kv_heads.  Scores, softmax statistics and sums are fp32; an fp16 output is
+ * within its own rounding of the exact one, as a rule; for a bf16 output V's
+ * scaled weights, and with more than 16 (token, head) rows per KV head K, V and
+ * the weights, are rounded to fp16 once.  A NaN in a key or value row reaches
+ * every token that sees the row, in its own dimensions or in all of them, and
+ * no other token.  Uses
+ * the context's attention scratch (39 MB): launches on one context are
+ * stream-ordered and must not overlap. */
 int mlm_attn_kv4(mlm_ctx *ctx, const mlm_kv4_cache *cache, const void *q_f16, int n_heads,
                  int tokens, const int32_t *len_dev, const int32_t *counts_dev, void *out,
                  int out_type);

@@ -44,6 +44,13 @@ constexpr int kD = kKv4D;
 // and sum per column.  Stretches of one head are joined in order: a warp's
 // pieces by their CTA, the CTAs' through the context's scratch by the last CTA of the
 // head to arrive, so sums do not depend on timing.
+//
+// Measured in a graph: 64 sequences x 8192 rows x 8 KV heads (673 MB) 117 us, 5.75 TB/s;
+// 131071 rows x 8 (168 MB) 44 us; 2048 rows 10 us, some 5 us of it the cut, the first
+// copies and the joins.  711 instructions per block of 32 rows, issue slots 60 % and the
+// ALU pipe (masks, transposes, conversions) 54 % busy on 24 ragged sequences.  Warps,
+// ring: 16 x 2 stages for 8 columns, 8 x 4 for 16 (the reverse: 139 us for the 64
+// sequences, 58 against 38 us for 8 x 4 tokens).
 // ---------------------------------------------------------------------------
 
 constexpr int kBlk = 32;                     // cache rows per block
