@@ -608,7 +608,8 @@ int mlm_llama_decode_greedy(mlm_llama *m, int token, int steps, int32_t *tokens_
 /* Sampled generation: mlm_llama_decode_greedy with mlm_sample_f32 in the argmax's
  * place.  `params` (host) holds the settings, uniforms_dev[i] (device, [steps]) the
  * i-th step's random number.  The settings and numbers are copied into the runner;
- * a call with others replays the same captured step. */
+ * a call with others replays the same captured step.  In a group every rank gives
+ * the same settings and numbers and draws the same tokens. */
 int mlm_llama_decode_sample(mlm_llama *m, int token, int steps, const mlm_sample_params *params,
                             const float *uniforms_dev, int32_t *tokens_out_dev);
 

@@ -5,7 +5,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from metallm_b200 import Llama, MLMError
+from metallm_b200 import Context, Llama, MLMError
 from metallm_b200.synthetic import fill_llama, llama_config
 from tests import kv4_reference as R
 
@@ -96,6 +96,15 @@ def test_decode_sample_batch(ctx):
         toks = [R.sample(x[b], *SETTINGS[b], us[s, b])[0] for b in range(B)]
         assert got[s].tolist() == toks, s
     m.close()
+
+
+def test_group_of_one_gathers_the_logits():
+    """A one-rank group takes the sharded path: the vocabulary's shards gathered, then sampled, alone
+    and as a batch, and its captured steps go before the group."""
+    with Context(0) as c:
+        c.tp_init(1, 0, c.tp_unique_id())
+        test_decode_sample_matches_sampling_the_logits(c)
+        test_decode_sample_batch(c)
 
 
 def test_refusals(ctx):
