@@ -947,6 +947,7 @@ extern "C" int mlm_llama_decode_sample(mlm_llama *m, int token, int steps,
   if (!m) return MLM_ERR_ARG;
   mlm_ctx *ctx = m->ctx;
   const char *what = "mlm_llama_decode_sample";
+  DeviceGuard guard(ctx);
   MLM_REQUIRE(ctx, tokens_out && steps > 0, MLM_ERR_ARG, "%s: no output", what);
   MLM_REQUIRE(ctx, token >= 0 && token < m->cfg.vocab, MLM_ERR_ARG, "%s: invalid token id %d", what,
               token);
@@ -979,6 +980,7 @@ extern "C" int mlm_llama_decode_sample_batch(mlm_llama *m, const int32_t *tokens
   if (!m) return MLM_ERR_ARG;
   mlm_ctx *ctx = m->ctx;
   const char *what = "mlm_llama_decode_sample_batch";
+  DeviceGuard guard(ctx);
   MLM_REQUIRE(ctx, tokens_out && steps > 0 && steps <= m->cfg.max_seq, MLM_ERR_ARG,
               "%s: no output, or steps=%d", what, steps);
   int st = batch_begin(m, tokens, steps, what);

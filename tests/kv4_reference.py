@@ -62,17 +62,19 @@ def attention(q, k_rows, v_rows, lens, counts):
     return out, smax, vmax
 
 
-def attention_tolerance(ref, smax, vmax, out_eps, rounded_operands):
+def attention_tolerance(ref, smax, vmax, out_eps, rounded_operands, rounded_weights=False):
     """Largest allowed |got - ref|.
 
     A score is a sum of 128 products: in 32 bits its error is below 128 roundings of
     2^-23 (tensor cores truncate) of sum |q k| / sqrt(128); where K is rounded to fp16
     first, 2^-11 of the same more.  An error e of every score moves the output by at
     most 2 e max|v| (1 + small).  exp, the sums and the division add 2^-18 of max|v|;
-    weights and V rounded to fp16 2^-11 of max|v| each.  The output itself is rounded by
-    at most half a step."""
+    weights and V rounded to fp16 2^-11 of max|v| each.  `rounded_weights`: the weights p and
+    then p d rounded to fp16, 2^-11 of p d c each, where d c is at most V's range, 2 max|v|.
+    The output itself is rounded by at most half a step."""
     e = smax * (128 * 2.0 ** -23 + (2.0 ** -11 if rounded_operands else 0))
     rel = np.expm1(2 * e) + 2.0 ** -18 + (2 * 2.0 ** -11 if rounded_operands else 0)
+    rel += 2 * 2 * 2.0 ** -11 if rounded_weights else 0
     return (out_eps / 2) * np.abs(ref) + (1 + out_eps) * rel * vmax + 2.0 ** -25
 
 
