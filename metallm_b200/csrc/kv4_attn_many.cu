@@ -41,6 +41,7 @@
 // masked weight is 0, but 0 x NaN is not, so a value row with NaN scales goes in
 // as zeros and makes its key NaN instead.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "kv4_common.cuh"
@@ -387,7 +388,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
       const int row = p.rt * kRows + tile * kTile + r;
       const bool mine = tile * kTile + r < live;
       const int tok = mine ? row / a.group : 0;
-      const int seen = mine ? max(0, p.len - p.count + tok + 1) : 0;
+      // (a row past the item sees all of its zero scores: the mask for its sake cost 64 rows
+      // x 16 sequences of 16000 296 us, 238 without)
+      const int seen = mine ? max(0, p.len - p.count + tok + 1) : INT_MAX;
       const size_t at = (((size_t)p.b * a.tokens + tok) * a.n_heads + p.h * a.group +
                          (row - tok * a.group)) * kKv4D;
       // Q in the order of the codes: half a warp per row
