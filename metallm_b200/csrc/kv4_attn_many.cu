@@ -728,11 +728,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
   }
 }
 
-// Joins the parts of items that several CTAs shared, in order: a CTA per 32 rows of
-// a KV head, a thread per four dimensions (8 rows of four dimensions are a line of a
-// part) of four rows, whose loads are in flight together.
-constexpr int kJoinRows = 32;
-template <class OutT>
+// Joins the parts of items that several CTAs shared, in order: a CTA per 8 ROWS rows
+// of a KV head, a thread per four dimensions (8 rows of four dimensions are a line of a
+// part) of ROWS rows, the loads of PARTS parts in flight together.
+template <class OutT, int ROWS, int PARTS>
 __global__ void __launch_bounds__(256) kv4_attn_join_kernel(Kv4AttnArgs a, int groups) {
   const int lane = threadIdx.x & 31;
   const int rg = blockIdx.x % groups, h = blockIdx.x / groups % a.n_kv;
@@ -742,7 +741,7 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(Kv4AttnArgs a, int g
   const long long quota = plan[0], first = plan[1 + b];
   int len, count;
   seq_shape(a, b, len, count);
-  const int row0 = rg * kJoinRows, rt = row0 / kRows;
+  const int row0 = rg * 8 * ROWS, rt = row0 / kRows;
   if (row0 >= count * a.group) return;
   const int nkt = key_tiles(len, count, a.group, rt);
   if (nkt == 0) return;
@@ -755,38 +754,47 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(Kv4AttnArgs a, int g
   if (c0 == c1) return;
   const int r = row0 - rt * kRows + (threadIdx.x & 7), c4 = threadIdx.x >> 3;
   auto part_of = [&](int c) { return a.parts + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kPartFloats; };
-  float top[4], sum[4] = {};
-  float4 v[4];
+  float top[ROWS], sum[ROWS] = {};
+  float4 v[ROWS];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < ROWS; ++i) {
     top[i] = -INFINITY;
     v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-#pragma unroll 2
-  for (int c = c0; c <= c1; ++c) {
-    const float *p = part_of(c);
-    float4 o[4];
-    float m[4], l[4];
+#pragma unroll 1
+  for (int c = c0; c <= c1; c += PARTS) {
+    float4 o[PARTS][ROWS];
+    float m[PARTS][ROWS], l[PARTS][ROWS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o[i] = reinterpret_cast<const float4 *>(p)[c4 * kRows + r + 8 * i];
-      m[i] = p[kRows * kKv4D + r + 8 * i];
-      l[i] = p[kRows * (kKv4D + 1) + r + 8 * i];
+    for (int k = 0; k < PARTS; ++k) {
+      const float *p = part_of(min(c + k, c1));
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        o[k][i] = reinterpret_cast<const float4 *>(p)[c4 * kRows + r + 8 * i];
+        m[k][i] = p[kRows * kKv4D + r + 8 * i];
+        l[k][i] = p[kRows * (kKv4D + 1) + r + 8 * i];
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float up = fmaxf(top[i], m[i]);
-      const float fo = top[i] == up ? 1.f : ex2(top[i] - up), f = m[i] == up ? 1.f : ex2(m[i] - up);
-      v[i].x = fmaf(f, o[i].x, v[i].x * fo);
-      v[i].y = fmaf(f, o[i].y, v[i].y * fo);
-      v[i].z = fmaf(f, o[i].z, v[i].z * fo);
-      v[i].w = fmaf(f, o[i].w, v[i].w * fo);
-      sum[i] = fmaf(f, l[i], sum[i] * fo);
-      top[i] = up;
+    for (int k = 0; k < PARTS; ++k) {
+      if (c + k > c1) break;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const float4 x = o[k][i];
+        const float up = fmaxf(top[i], m[k][i]);
+        const float fo = top[i] == up ? 1.f : ex2(top[i] - up),
+                    f = m[k][i] == up ? 1.f : ex2(m[k][i] - up);
+        v[i].x = fmaf(f, x.x, v[i].x * fo);
+        v[i].y = fmaf(f, x.y, v[i].y * fo);
+        v[i].z = fmaf(f, x.z, v[i].z * fo);
+        v[i].w = fmaf(f, x.w, v[i].w * fo);
+        sum[i] = fmaf(f, l[k][i], sum[i] * fo);
+        top[i] = up;
+      }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < ROWS; ++i) {
     const int row = rt * kRows + r + 8 * i;
     if (row >= count * a.group) continue;
     const int t = row / a.group;
@@ -806,11 +814,16 @@ int many(mlm_ctx *ctx, const Kv4AttnArgs &a) {
                                              dim3(kThreads), smem_bytes(a.batch), ctx->stream, a),
                                   "mlm_attn_kv4");
   if (st != MLM_OK) return st;
-  const int groups = (a.tokens * a.group + kJoinRows - 1) / kJoinRows;
+  const int rows = a.tokens * a.group;
+  // Short of a CTA per SM the rows have many parts each: 8 rows per CTA, 8 parts at a time
+  // (8 tokens at 2000 rows, 32/8 heads: 18.3 us, 28.2 with 32 rows); else 32 rows (1024
+  // tokens at 8192: 147 us, 160 with 8)
+  const bool few = (long long)((rows + 31) / 32) * a.n_kv * a.batch < ctx->sm_count;
+  const int groups = few ? (rows + 7) / 8 : (rows + 31) / 32;
   return check_launch_pdl(
       ctx,
-      launch_pdl(kv4_attn_join_kernel<OutT>, dim3((unsigned)groups * a.n_kv * a.batch),
-                 dim3(256), 0, ctx->stream, a, groups),
+      launch_pdl(few ? kv4_attn_join_kernel<OutT, 1, 8> : kv4_attn_join_kernel<OutT, 4, 2>,
+                 dim3((unsigned)groups * a.n_kv * a.batch), dim3(256), 0, ctx->stream, a, groups),
       "mlm_attn_kv4 (join)");
 }
 
