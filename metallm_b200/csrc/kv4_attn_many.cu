@@ -31,7 +31,7 @@
 // that several CTAs share leaves fp32 parts in the context's scratch, which a
 // second kernel joins in order.
 //
-// Measured in a graph: 1024 tokens at 8192, 32/8 heads, 149 us, 862 TFLOP/s, the tensor
+// Measured in a graph: 1024 tokens at 8192, 32/8 heads, 148 us, 870 TFLOP/s, the tensor
 // pipe 44 % active: bound by the chain S, softmax, P, P V of the two row tiles (144 us
 // without exponentials, maxima and dequantization, 107 us without the products).  Half
 // tiles with a thread per row tile issuing took 167 us, handing P over in halves 170,
