@@ -58,11 +58,12 @@ constexpr int kHalfStage = kBlk * kRow;      // K or V of a block
 constexpr int kStage = 2 * kHalfStage;
 constexpr int kPieceRow = kD + 4;            // a column of a piece: o[128], m, l, padding
 constexpr int kMaxCols = 16;
-// Weights are 2^(s - max + bias), a score at most 2^kLead above the maximum, and p d has
-// to be an fp16 value: with V's scales below 2 up to 2^15, else (d < 2^13.1, the largest
-// that the append writes) up to 2^14.1.  A weight 2^24 times smaller than the largest still
-// keeps the bits of its hi part and lo part that a long cache's sum needs.
-constexpr float kLead = 4.f, kBias = 10.f, kBiasWide = -3.f;
+// Weights are 2^(s - max + kBias), a score at most 2^kLead above the maximum, so p is below
+// 2^14; d goes in scaled by a power of two per group that brings the largest of the item so
+// far into [1, 2), so p d is below 2^15.  Both are then held to 2^-25, 2^-35 of the largest
+// weight (times the largest scale), which is what the many small weights behind a large one
+// need: 2^17 rows add up to 2^-18 at most that way.
+constexpr float kLead = 4.f, kBias = 10.f;
 
 // a product from zero accumulators
 __device__ __forceinline__ void mma_f16_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -171,6 +172,14 @@ template <bool EXACT>
 __device__ __forceinline__ float code_unit(int i) {
   return EXACT ? 1048576.f : (i & 1) ? 262144.f : 4194304.f;
 }
+
+// The unit 2^e, -15 <= e <= 15, that V's scales of a group are counted in: its reciprocal,
+// a binary16 value twice, by which they are multiplied
+__device__ __forceinline__ uint32_t unit_of(int e) {
+  return (e < 15 ? (uint32_t)(15 - e) << 10 : 0x0200u) * 0x10001u;
+}
+__device__ __forceinline__ int unit_exponent(uint32_t unit) { return 15 - (int)((unit & 0xFFFFu) >> 10); }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // an item (the blocks of one KV head of one sequence) and a block of it
 struct Item {
@@ -408,7 +417,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
   int seen[NT];                // rows column r attends to
   uint32_t qm[NT][2];          // the B operand of K's minima: (0, group sum) per group, hi and lo
   float o[NT][4][2][4], mx[NT], l[NT];
-  float bias = kBias;          // of the weights' exponent: kBiasWide once a V scale is 2 or more
+  uint32_t unit = 0;           // even r: what V's scales of group r / 2 are multiplied by, twice
   float om[NT][4];             // sum of p m: rows 2 g + 1 of the product with V's scales
   bool ok = true;
   int stage = 0;
@@ -423,7 +432,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
       const Item cur = s_cur[warp];
       const int len = cur.len, count = cur.count;
       mask_from = max(0, len - count + 1) / kBlk;
-      bias = kBias;
+      unit = r & 1 ? 0x3C003C00u : 0x78007800u;  // 1, and 2^15 until the first block's scales are known
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int col = DUP ? (r & 3) : nt * 8 + r;
@@ -560,33 +569,49 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
         const uint32_t bits = good >> (4 * kt + 2 * j);
         return ((bits & 1) ? 0xFFFFu : 0u) | ((bits & 2) ? 0xFFFF0000u : 0u);
       };
-      // V's transposed scale words: d in the lanes of even r, m in the others.  A scale of
-      // 2 or more has bit 14 set
+      // V's transposed scale words: d in the lanes of even r, in the group's unit, m in the
+      // others.  A scale of 2 units or more has bit 14 set
       uint32_t mt[2][2];
+      auto value_scales = [&] {
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        ldsm2_t(sv + (kt * 16 + (lane & 15)) * kRow + 64, mt[kt]);
-        if (MASK) {
-          mt[kt][0] &= good_pair(kt, 0);
-          mt[kt][1] &= good_pair(kt, 1);
-        }
-      }
-      {
-        const uint32_t bits = (mt[0][0] | mt[0][1] | mt[1][0] | mt[1][1]) & (r & 1 ? 0u : 0x40004000u);
-        if (__any_sync(0xffffffffu, bits != 0) && bias == kBias) {
-          const float f = 1.f / (1 << (int)(kBias - kBiasWide));
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            l[nt] *= f;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              om[nt][g] *= f;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) o[nt][g][0][i] *= f, o[nt][g][1][i] *= f;
-            }
+        for (int kt = 0; kt < 2; ++kt) {
+          ldsm2_t(sv + (kt * 16 + (lane & 15)) * kRow + 64, mt[kt]);
+          if (MASK) {
+            mt[kt][0] &= good_pair(kt, 0);
+            mt[kt][1] &= good_pair(kt, 1);
           }
-          bias = kBiasWide;
         }
+      };
+      auto to_units = [&] {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) mt[kt][j] = hmul2(mt[kt][j], unit);
+      };
+      value_scales();
+      to_units();
+      const uint32_t any_d = mt[0][0] | mt[0][1] | mt[1][0] | mt[1][1];
+      if (__any_sync(0xffffffffu, (any_d & (r & 1 ? 0u : 0x40004000u)) != 0)) {
+        // larger scales than before (or infinities, NaN): larger units, what has been
+        // summed scaled to them
+        value_scales();
+        uint32_t big = __vmaxu2(__vmaxu2(mt[0][0] & 0x7FFF7FFFu, mt[0][1] & 0x7FFF7FFFu),
+                                __vmaxu2(mt[1][0] & 0x7FFF7FFFu, mt[1][1] & 0x7FFF7FFFu));
+        big = max(big & 0xFFFFu, big >> 16);
+        big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        const int was = unit_exponent(unit);
+        const int now = r & 1 ? was : max(was, min((int)(big >> 10) - 15, 15));
+        unit = unit_of(now);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float f = power_of_two(__shfl_sync(0xffffffffu, was - now, 8 * g));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[nt][g][0][i] *= f, o[nt][g][1][i] *= f;
+        }
+        to_units();
       }
       // Running maximum and sum.  The maximum follows only when a score leads it
       // by more than 2^kLead; the factor is l's too.
@@ -616,7 +641,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
           }
           mx[nt] = top;
         }
-        const float base = fmaf(mx[nt] == -INFINITY ? 0.f : mx[nt], -cs[nt], bias);
+        const float base = fmaf(mx[nt] == -INFINITY ? 0.f : mx[nt], -cs[nt], kBias);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float &v = sT[nt][i >> 2][(i >> 1) & 1][i & 1];
@@ -671,7 +696,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
           for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              // d of rows 2 t4, + 1 (and of rows 2 t4 + 8, + 9)
+              // d of rows 2 t4, + 1 (and of rows 2 t4 + 8, + 9), in units
               const uint32_t d = __shfl_sync(0xffffffffu, mt[kt][j], 8 * g + t4);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
@@ -752,6 +777,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
             m0 += __shfl_xor_sync(0xffffffffu, m0, 2);
             m1 += __shfl_xor_sync(0xffffffffu, m1, 2);
           }
+          const float in_units = power_of_two(__shfl_sync(0xffffffffu, unit_exponent(unit), 8 * g));
           float v[2][4];  // columns 2 t4 and 2 t4 + 1, dimensions 32 g + 4 r ..
 #pragma unroll
           for (int i = 0; i < 2; ++i)
@@ -759,7 +785,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
             for (int c = 0; c < 4; ++c) {
               float w = o[nt][g][i][c];
               if (kSplit) w += __shfl_xor_sync(0xffffffffu, w, 2);  // hi + lo
-              v[c & 1][2 * i + (c >> 1)] = fmaf(w, code_unit<LO>(c >> 1), (c & 1) ? m1 : m0);
+              v[c & 1][2 * i + (c >> 1)] = fmaf(w, code_unit<LO>(c >> 1) * in_units, (c & 1) ? m1 : m0);
             }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -785,7 +811,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
           }
         }
         if (!whole && t4 == 0 && (!DUP || r < 4)) {
-          piece[(nt * 8 + r) * kPieceRow + kD] = fmaf(mx[nt], cs[nt], -bias);
+          piece[(nt * 8 + r) * kPieceRow + kD] = fmaf(mx[nt], cs[nt], -kBias);
           piece[(nt * 8 + r) * kPieceRow + kD + 1] = l[nt];
         }
       }

@@ -1,0 +1,98 @@
+"""Attention over the 4-bit cache where its precision is at stake: small weights beside large ones."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from metallm_b200 import TYPE_BF16, TYPE_F16, Kv4Cache
+from tests import kv4_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+def _parts(rows):
+    """m and d c of cache rows [..., 80], in 64 bits: [..., 128] each."""
+    zero = rows.copy()
+    zero[..., :64] = 0
+    m = R.values(zero)
+    return m, R.values(rows) - m
+
+
+def _attend(ctx, k_rows, v_rows, batch, q, out_type):
+    """q [batch][tokens][heads][128] over `batch` copies of one KV head's rows [n][80]."""
+    import torch
+    n = k_rows.shape[0]
+    dk, dv = (torch.from_numpy(r).cuda().expand(batch, n, R.ROW).contiguous() for r in (k_rows, v_rows))
+    lens = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    dq = torch.from_numpy(q).cuda()
+    out = torch.zeros(q.shape, dtype=torch.float16 if out_type == TYPE_F16 else torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    ctx.attn_kv4(Kv4Cache(dk.data_ptr(), dv.data_ptr(), batch, 1, R.D, n), dq.data_ptr(), q.shape[2],
+                 q.shape[1], lens.data_ptr(), None, out.data_ptr(), out_type)
+    ctx.wait()
+    return out.double().cpu().numpy()
+
+
+# ---- small weights beside large ones -------------------------------------------
+
+N_PEAKED, PERIOD = 32768, 8192
+V_KINDS = {
+    "one": lambda x, j: x,
+    "small": lambda x, j: x * 0.002,
+    # one group spans 30 and more, the others do not
+    "wide": lambda x, j: np.concatenate([x[:, :96], x[:, 96:] * 60], 1),
+    # single rows of 40 times the others' scale, in two groups
+    "late": lambda x, j: np.where((j % 997 == 500)[:, None] & (np.arange(R.D) >= 64), x * 40, x),
+}
+
+
+@pytest.fixture(scope="module", params=list(V_KINDS))
+def peaked(request):
+    """Keys of which every 8192nd outweighs the others by as many octaves as the query says, and whose
+    own value row is zero: the outputs are what the small weights add up to."""
+    rng = np.random.default_rng(7)
+    j = np.arange(N_PEAKED)
+    k = 0.3 * rng.standard_normal((N_PEAKED, R.D)).astype(np.float32)
+    v = (1 + 0.3 * rng.standard_normal((N_PEAKED, R.D))).astype(np.float32)
+    v = V_KINDS[request.param](v, j).astype(np.float32)
+    peak = j % PERIOD == 0
+    k[:, 0] = np.where(peak, 8, 0)
+    v[peak] = 0
+    return R.quantize(k), R.quantize(v)
+
+
+@pytest.mark.parametrize("out_type", [TYPE_F16, TYPE_BF16])
+@pytest.mark.parametrize("heads", [4, 8, 16])
+def test_small_weights_beside_large_ones(ctx, peaked, heads, out_type):
+    """1024 sequences, so that a warp walks thousands of rows behind a dominant key."""
+    k_rows, v_rows = peaked
+    rng = np.random.default_rng(heads)
+    q = 0.05 * rng.standard_normal((1, 1, heads, R.D))
+    q[0, 0, :, 0] = np.linspace(15.3, 25.6, heads) * np.log(2) * np.sqrt(R.D) / 8  # octaves
+    q = q.astype(np.float16)
+    batch = 1024
+    got = _attend(ctx, k_rows, v_rows, batch, np.repeat(q, batch, axis=0), out_type)[:, 0]
+
+    x = q[0, 0].astype(np.float64)
+    k, (m, dc) = R.values(k_rows), _parts(v_rows)
+    s = x @ k.T / np.sqrt(R.D)
+    p = np.exp(s - s.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    ref = p @ (m + dc)
+    # An error e of every score moves a weight by its expm1(e) at most, the sum of them too: 2 e of the
+    # mean |v|.  A score's is 128 roundings of 2^-23 of sum |q k|.  exp and the sums: 2^-18.
+    bf16 = out_type == TYPE_BF16
+    smax = (np.abs(x) @ np.abs(k).T).max(1, keepdims=True) / np.sqrt(R.D)
+    e = smax * 128 * 2.0 ** -23
+    mean_m, mean_dc = p @ np.abs(m), p @ np.abs(dc)
+    tol = (np.expm1(2 * e) + 2.0 ** -18) * (mean_m + mean_dc)
+    # to bf16 the weights are fp16 values (2^-11), then p d once more
+    if bf16:
+        tol += 2.0 ** -11 * (mean_m + 2 * mean_dc) * (1 + 2.0 ** -8)
+    # a weight (and a p d, of the largest d) is held to 2^-25 where the largest weight is 2^10 or more
+    vmax = (np.abs(m).reshape(-1, 4, 32) + 15 / 7.5 * np.abs(dc).reshape(-1, 4, 32)).max((0, 2)).repeat(32)
+    tol += 2 * N_PEAKED * 2.0 ** -35 * vmax
+    tol += (2.0 ** -8 if bf16 else 2.0 ** -11) * (np.abs(ref) + tol) + 2.0 ** -25
+    over = np.abs(got - ref) / tol
+    at = np.unravel_index(over.argmax(), over.shape)
+    assert over.max() <= 1, (at, got[at], ref[at[1:]], over.max())
