@@ -642,12 +642,14 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
           mx[nt] = top;
         }
         const float base = fmaf(mx[nt] == -INFINITY ? 0.f : mx[nt], -cs[nt], kBias);
+        float sum = 0.f;  // the block's first: thousands of equal weights one by one are rounded alike
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float &v = sT[nt][i >> 2][(i >> 1) & 1][i & 1];
           v = ex2(fmaf(v, cs[nt], base));
-          l[nt] += v;
+          sum = i == 0 ? v : sum + v;
         }
+        l[nt] += sum;
       }
       // the weights of the lane's eight rows as fp16 hi (and lo) pairs, and the m part:
       // sum_j p_j m_jg (and p_j d_jg, unused)

@@ -13,13 +13,19 @@
 //   - 4 warps per row tile do the softmax, a thread per row: S from TMEM, the
 //     weights back as fp16 over it, where the second product reads them as its A
 //     operand.
-// The running maximum follows only when a score leads it by more than 2^12, so the
-// accumulator in TMEM is rescaled once in a row's life, as a rule.  The weights are
-// 2^(s - max + 3): at most 2^15, and fp16 values of full precision down to 2^-17 of the
-// maximum's, as the many small ones of a long cache want.  Scores, maxima and sums are
-// fp32.  For a bf16 output K, V and the weights are fp16 operands, each rounded once; an
-// fp16 output, eight times finer, would show that (up to three times its own rounding),
-// so there each is hi + lo: two products for the scores, three for O.
+// The running maximum follows only when a score leads it by more than 2^8, so the
+// accumulator in TMEM is rescaled once or twice in a row's life, as a rule.  The weights
+// are 2^(s - max + 7): at most 2^15, and held to 2^-32 of the largest, as the many small
+// ones of a long cache want (2^17 of them are off by 2^-15 together).  Scores, maxima and
+// sums are fp32.  For a bf16 output K, V and the weights are fp16 operands, each rounded
+// once; an fp16 output, eight times finer, would show that (up to three times its own
+// rounding), so there each is hi + lo: two products for the scores, three for O.
+//
+// A product's accumulators are cut off, not rounded, by up to 2^-23 each time, and 131072
+// keys in one accumulator shrank by 4e-4.  So after 128 key tiles (512 for a bf16 output)
+// O is added to the part of the scratch that the item would leave, and the next products
+// start from zero.  All CTAs at once move 38 MB each way in such a fold, some 10 us: every
+// 64 tiles 1024 tokens at 32768 keys to bf16 took 558 us, 520 as it is.
 //
 // V^T is the N-major B operand of the second product: both K and V lie in
 // shared memory as [key][dimension] in the 128-byte swizzle, the eight
@@ -73,7 +79,9 @@ constexpr size_t smem_bytes(int batch) { return kOffLine + 8 * (size_t)(batch + 
 constexpr int kTmemCols = 512;  // S/P of tile 0 and 1, O of tile 0 and 1
 constexpr int kPartFloats = kRows * (kKv4D + 2);  // o, then m and l
 constexpr float kScale2 = kInvSqrtD * kLog2e;
-constexpr float kBias = 3.f, kLead = 12.f / kScale2;
+constexpr float kBias = 7.f, kLead = 8.f / kScale2;
+// key tiles whose products O sums in TMEM: 24 products a tile for an fp16 output, 8 for bf16
+constexpr int fold_of(bool exact) { return exact ? 128 : 512; }
 
 // instruction descriptors: fp16 A and B, fp32 accumulators, M = N = 128; B K-major
 // (S = Q K^T) or N-major (O = P V)
@@ -304,6 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
   // hi + lo operands, each in one buffer of the two instead of one in two
   constexpr bool EXACT = std::is_same<OutT, __half>::value;
   constexpr uint32_t kStages = EXACT ? 1 : 2;
+  constexpr int kFold = fold_of(EXACT);
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = (uint32_t)__cvta_generic_to_shared(smem);
   const uint32_t bar = sbase + kOffBar;
@@ -420,116 +429,162 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
         continue;
       }
       ++n_q;
+      // the CTA's part of the item: [4 columns][row], then the rows' maxima and sums.  An
+      // item without parts folds into the second, which only the stretch's last item may
+      // leave.  (Found anew where it is used: the loop has no registers to spare.)
+      auto part_at = [&] {
+        const long long item = walk.x - p.kt1;  // the item's first tile on the line
+        return a.parts + ((size_t)blockIdx.x * 2 + (item < x0 ? 0 : 1)) * kPartFloats + 4 * (tile * kTile + r);
+      };
+      auto fold = [&](bool more, float m) {
+        float4 *part_o = reinterpret_cast<float4 *>(part_at());
+        float *part_m = reinterpret_cast<float *>(part_o) + kRows * kKv4D - 3 * (tile * kTile + r);
+        const float was = more ? *part_m : m;
+        const float f = was == m ? 1.f : ex2((was - m) * kScale2);
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(to + 32 * c, o);
+          tmem_wait_ld(o);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float4 *dst = part_o + (8 * c + j) * kRows;
+            const float4 x = more ? *dst : make_float4(0.f, 0.f, 0.f, 0.f);
+            *dst = make_float4(fmaf(f, x.x, __uint_as_float(o[4 * j])),
+                               fmaf(f, x.y, __uint_as_float(o[4 * j + 1])),
+                               fmaf(f, x.z, __uint_as_float(o[4 * j + 2])),
+                               fmaf(f, x.w, __uint_as_float(o[4 * j + 3])));
+          }
+        }
+        *part_m = m;
+      };
       float m = -INFINITY;
       uint64_t l2 = 0;
-      for (int kt = p.kt0; kt < p.kt1; ++kt) {
-        ok = __all_sync(0xffffffffu,
-                        mbar_wait_bounded(bar + 8 * (kSfull + tile), n_s & 1, a.status));
-        if (!ok) break;
-        ++n_s;
-        tc_fence_after();
-        const int lim = seen - kt * kTile;  // keys of the tile that the row sees
-        auto weights = [&](auto mask_tag) {
-          constexpr bool MASK = decltype(mask_tag)::value;
-          uint32_t s[2][32];
-          float m2 = m == -INFINITY ? 0.f : fmaf(-m, kScale2, kBias);
-          tmem_ld32(ts, s[0]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t(&v)[32] = s[c & 1];
-            tmem_wait_ld(v);
-            if (c < 3) tmem_ld32(ts + 32 * (c + 1), s[(c + 1) & 1]);
-            float top = -INFINITY, top1 = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              if (MASK) {
-                if (32 * c + k >= lim) v[k] = 0xFF800000u;
-                if (32 * c + k + 1 >= lim) v[k + 1] = 0xFF800000u;
-              }
-              top = fmaxf(top, __uint_as_float(v[k]));
-              top1 = fmaxf(top1, __uint_as_float(v[k + 1]));
-            }
-            top = fmaxf(top, top1);
-            if (__any_sync(0xffffffffu, top > m + kLead)) {
-              // a new maximum: what has been summed against the old one is scaled,
-              // O, l and this tile's weights so far
-              if (c < 3) tmem_wait_ld(s[(c + 1) & 1]);
-              const float up = fmaxf(m, top);
-              const float f = up == m ? 1.f : ex2((m - up) * kScale2);
-              if (kt > p.kt0) {
-#pragma unroll 1
-                for (int j = 0; j < 4; ++j) {
-                  uint32_t o[32];
-                  tmem_ld32(to + 32 * j, o);
-                  tmem_wait_ld(o);
-#pragma unroll
-                  for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                  tmem_st32(to + 32 * j, o);
+      for (int first = p.kt0; first < p.kt1; first += kFold) {
+        const int last = min(p.kt1, first + kFold);
+        if (first > p.kt0) {
+          // The sums of the last kFold tiles, in the order of the products, are added to
+          // those before; once the next S is there they are complete
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait_bounded(bar + 8 * (kSfull + tile), n_s & 1, a.status));
+          if (!ok) break;
+          tc_fence_after();
+          fold(first - p.kt0 > kFold, m);
+        }
+        for (int kt = first; kt < last; ++kt) {
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait_bounded(bar + 8 * (kSfull + tile), n_s & 1, a.status));
+          if (!ok) break;
+          ++n_s;
+          tc_fence_after();
+          const int lim = seen - kt * kTile;  // keys of the tile that the row sees
+          auto weights = [&](auto mask_tag) {
+            constexpr bool MASK = decltype(mask_tag)::value;
+            uint32_t s[2][32];
+            float m2 = m == -INFINITY ? 0.f : fmaf(-m, kScale2, kBias);
+            tmem_ld32(ts, s[0]);
+  #pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t(&v)[32] = s[c & 1];
+              tmem_wait_ld(v);
+              if (c < 3) tmem_ld32(ts + 32 * (c + 1), s[(c + 1) & 1]);
+              float top = -INFINITY, top1 = -INFINITY;
+  #pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                if (MASK) {
+                  if (32 * c + k >= lim) v[k] = 0xFF800000u;
+                  if (32 * c + k + 1 >= lim) v[k + 1] = 0xFF800000u;
                 }
+                top = fmaxf(top, __uint_as_float(v[k]));
+                top1 = fmaxf(top1, __uint_as_float(v[k + 1]));
               }
-              tmem_wait_st();
-              if (EXACT) {
-#pragma unroll 1
-                for (int j = 0; j < c; ++j) {
-                  uint32_t o[32];
-                  tmem_ld32(ts + 32 * j, o);
-                  tmem_wait_ld(o);
-#pragma unroll
-                  for (int k = 0; k < 16; ++k) {
-                    const float2 h = unpack_f16(o[k]), e = unpack_f16(o[16 + k]);
-                    split_f16((h.x + e.x) * f, (h.y + e.y) * f, o[k], o[16 + k]);
+              top = fmaxf(top, top1);
+              if (__any_sync(0xffffffffu, top > m + kLead)) {
+                // a new maximum: what has been summed against the old one is scaled,
+                // O, l and this tile's weights so far
+                if (c < 3) tmem_wait_ld(s[(c + 1) & 1]);
+                const float up = fmaxf(m, top);
+                const float f = up == m ? 1.f : ex2((m - up) * kScale2);
+                if (kt > first) {
+  #pragma unroll 1
+                  for (int j = 0; j < 4; ++j) {
+                    uint32_t o[32];
+                    tmem_ld32(to + 32 * j, o);
+                    tmem_wait_ld(o);
+  #pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                    tmem_st32(to + 32 * j, o);
                   }
-                  tmem_st32(ts + 32 * j, o);
                 }
-              } else {
-#pragma unroll 1
-                for (int j = 0; j < (c + 1) / 2; ++j) {  // 64 weights at a time
-                  uint32_t o[32];
-                  tmem_ld32(ts + 32 * j, o);
-                  tmem_wait_ld(o);
-                  uint32_t h[16];
-#pragma unroll
-                  for (int half = 0; half < 2; ++half) {
-#pragma unroll
+                tmem_wait_st();
+                if (EXACT) {
+  #pragma unroll 1
+                  for (int j = 0; j < c; ++j) {
+                    uint32_t o[32];
+                    tmem_ld32(ts + 32 * j, o);
+                    tmem_wait_ld(o);
+  #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                      const float2 e = unpack_f16(o[16 * half + k]);
-                      h[k] = pack_f16(e.x * f, e.y * f);
+                      const float2 h = unpack_f16(o[k]), e = unpack_f16(o[16 + k]);
+                      split_f16((h.x + e.x) * f, (h.y + e.y) * f, o[k], o[16 + k]);
                     }
-                    if (2 * j + half < c) tmem_st16(ts + 32 * j + 16 * half, h);
+                    tmem_st32(ts + 32 * j, o);
+                  }
+                } else {
+  #pragma unroll 1
+                  for (int j = 0; j < (c + 1) / 2; ++j) {  // 64 weights at a time
+                    uint32_t o[32];
+                    tmem_ld32(ts + 32 * j, o);
+                    tmem_wait_ld(o);
+                    uint32_t h[16];
+  #pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+  #pragma unroll
+                      for (int k = 0; k < 16; ++k) {
+                        const float2 e = unpack_f16(o[16 * half + k]);
+                        h[k] = pack_f16(e.x * f, e.y * f);
+                      }
+                      if (2 * j + half < c) tmem_st16(ts + 32 * j + 16 * half, h);
+                    }
                   }
                 }
+                tmem_wait_st();
+                const float2 l = unpair(l2);
+                l2 = pair(l.x * f, l.y * f);
+                m = up;
+                m2 = m == -INFINITY ? 0.f : fmaf(-m, kScale2, kBias);
               }
-              tmem_wait_st();
-              const float2 l = unpair(l2);
-              l2 = pair(l.x * f, l.y * f);
-              m = up;
-              m2 = m == -INFINITY ? 0.f : fmaf(-m, kScale2, kBias);
+              const uint64_t mm = pair(m2, m2), cc = pair(kScale2, kScale2);
+              uint32_t w[16], rest[16];
+              // (a chunk's sum first: 2^16 equal weights added one by one would be rounded the
+              // same way each, by up to 2^-9 of a weight)
+              uint64_t sum2 = 0;
+  #pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                const float2 e =
+                    unpair(fma2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), cc, mm));
+                const float p0 = ex2(e.x), p1 = ex2(e.y);
+                sum2 = k == 0 ? pair(p0, p1) : add2(sum2, pair(p0, p1));
+                if (EXACT)
+                  split_f16(p0, p1, w[k / 2], rest[k / 2]);
+                else
+                  w[k / 2] = pack_f16(p0, p1);
+              }
+              l2 = add2(l2, sum2);
+              // over scores that have been read
+              tmem_st16(ts + (EXACT ? 32 : 16) * c, w);
+              if (EXACT) tmem_st16(ts + 32 * c + 16, rest);
             }
-            const uint64_t mm = pair(m2, m2), cc = pair(kScale2, kScale2);
-            uint32_t w[16], rest[16];
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              const float2 e =
-                  unpair(fma2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), cc, mm));
-              const float p0 = ex2(e.x), p1 = ex2(e.y);
-              l2 = add2(l2, pair(p0, p1));
-              if (EXACT)
-                split_f16(p0, p1, w[k / 2], rest[k / 2]);
-              else
-                w[k / 2] = pack_f16(p0, p1);
-            }
-            // over scores that have been read
-            tmem_st16(ts + (EXACT ? 32 : 16) * c, w);
-            if (EXACT) tmem_st16(ts + 32 * c + 16, rest);
-          }
-        };
-        if (__any_sync(0xffffffffu, lim < kTile))
-          weights(std::true_type());
-        else
-          weights(std::false_type());
-        tmem_wait_st();
-        tc_fence_before();
-        arrive(bar + 8 * (kPfull + tile));
+          };
+          if (__any_sync(0xffffffffu, lim < kTile))
+            weights(std::true_type());
+          else
+            weights(std::false_type());
+          tmem_wait_st();
+          tc_fence_before();
+          arrive(bar + 8 * (kPfull + tile));
+        }
+        if (!ok) break;
       }
       if (!ok) break;
       ok = __all_sync(0xffffffffu,
@@ -539,16 +594,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
       tc_fence_after();
       const float2 l = unpair(l2);
       const float sum = l.x + l.y;
-      const long long item = walk.x - p.kt1;  // the item's first tile on the line
       const bool whole = p.kt0 == 0 && p.kt1 == p.nkt;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      // parts: [4 columns][row], then the rows' maxima and sums
-      float *part = a.parts + ((size_t)blockIdx.x * 2 + (item < x0 ? 0 : 1)) * kPartFloats;
+      float4 *part_o = reinterpret_cast<float4 *>(part_at());
+      float *part_m = reinterpret_cast<float *>(part_o) + kRows * kKv4D - 3 * (tile * kTile + r);
+      const bool folded = p.kt1 - p.kt0 > kFold;
+      const float was = folded ? *part_m : m;
+      const float f_was = was == m ? 1.f : ex2((was - m) * kScale2);
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
         tmem_ld32(to + 32 * c, o);
         tmem_wait_ld(o);
+        if (folded) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 x = part_o[(8 * c + j) * kRows];
+            o[4 * j] = __float_as_uint(fmaf(f_was, x.x, __uint_as_float(o[4 * j])));
+            o[4 * j + 1] = __float_as_uint(fmaf(f_was, x.y, __uint_as_float(o[4 * j + 1])));
+            o[4 * j + 2] = __float_as_uint(fmaf(f_was, x.z, __uint_as_float(o[4 * j + 2])));
+            o[4 * j + 3] = __float_as_uint(fmaf(f_was, x.w, __uint_as_float(o[4 * j + 3])));
+          }
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float e[8];  // columns 0 4 1 5 2 6 3 7 back in order
@@ -561,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
             *reinterpret_cast<uint4 *>(s_q + chunk_at(r, 4 * c + j)) =
                 *reinterpret_cast<const uint4 *>(h);
           } else {
-            float4 *dst = reinterpret_cast<float4 *>(part) + (8 * c + 2 * j) * kRows + tile * kTile + r;
+            float4 *dst = part_o + (8 * c + 2 * j) * kRows;
             dst[0] = make_float4(e[0], e[1], e[2], e[3]);
             dst[kRows] = make_float4(e[4], e[5], e[6], e[7]);
           }
@@ -579,8 +646,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
         }
         __syncwarp();
       } else {
-        part[kRows * kKv4D + tile * kTile + r] = m * kScale2;
-        part[kRows * (kKv4D + 1) + tile * kTile + r] = sum;
+        part_m[0] = m * kScale2;
+        part_m[kRows] = sum;
       }
     }
   } else if (warp < kMmaWarp) {
@@ -688,7 +755,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
           if (!ok) break;
           ++n_p[i];
           tc_fence_after();
-          mma_tmem(tmem + (2 + i) * kTile, tmem + i * kTile, vb, kt > p.kt0);
+          mma_tmem(tmem + (2 + i) * kTile, tmem + i * kTile, vb, (kt - p.kt0) % kFold != 0);
           if (EXACT) {  // 32 weights' hi, then their lo
 #pragma unroll
             for (int k = 0; k < 8; ++k) {

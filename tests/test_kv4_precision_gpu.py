@@ -1,4 +1,5 @@
-"""Attention over the 4-bit cache where its precision is at stake: small weights beside large ones."""
+"""Attention over the 4-bit cache where its precision is at stake: small weights beside large
+ones, long stretches of a cache walked by one CTA."""
 from __future__ import annotations
 
 import numpy as np
@@ -62,7 +63,7 @@ def peaked(request):
 
 
 @pytest.mark.parametrize("out_type", [TYPE_F16, TYPE_BF16])
-@pytest.mark.parametrize("heads", [4, 8, 16])
+@pytest.mark.parametrize("heads", [4, 8, 16, 32])
 def test_small_weights_beside_large_ones(ctx, peaked, heads, out_type):
     """1024 sequences, so that a warp walks thousands of rows behind a dominant key."""
     k_rows, v_rows = peaked
@@ -80,19 +81,64 @@ def test_small_weights_beside_large_ones(ctx, peaked, heads, out_type):
     p /= p.sum(1, keepdims=True)
     ref = p @ (m + dc)
     # An error e of every score moves a weight by its expm1(e) at most, the sum of them too: 2 e of the
-    # mean |v|.  A score's is 128 roundings of 2^-23 of sum |q k|.  exp and the sums: 2^-18.
+    # mean |v|.  A score's is 128 roundings of 2^-23 of sum |q k|; the many-row form to bf16 rounds K to
+    # fp16, 2^-11 of it.  exp and the sums: 2^-18.
+    many = heads > 16
     bf16 = out_type == TYPE_BF16
     smax = (np.abs(x) @ np.abs(k).T).max(1, keepdims=True) / np.sqrt(R.D)
-    e = smax * 128 * 2.0 ** -23
+    e = smax * (128 * 2.0 ** -23 + (2.0 ** -11 if many and bf16 else 0))
     mean_m, mean_dc = p @ np.abs(m), p @ np.abs(dc)
     tol = (np.expm1(2 * e) + 2.0 ** -18) * (mean_m + mean_dc)
-    # to bf16 the weights are fp16 values (2^-11), then p d once more
+    # to bf16 the weights are fp16 values (2^-11), then few rows' p d and many rows' V once more
     if bf16:
-        tol += 2.0 ** -11 * (mean_m + 2 * mean_dc) * (1 + 2.0 ** -8)
-    # a weight (and a p d, of the largest d) is held to 2^-25 where the largest weight is 2^10 or more
+        tol += 2.0 ** -11 * (mean_m + 2 * mean_dc) * (1 + 2.0 ** -8) + (2.0 ** -11 * mean_m if many else 0)
+    # a weight (and a p d, of the largest d) is held to 2^-25 where the largest weight is 2^10 or more; 2^7
+    # or more with many rows
     vmax = (np.abs(m).reshape(-1, 4, 32) + 15 / 7.5 * np.abs(dc).reshape(-1, 4, 32)).max((0, 2)).repeat(32)
-    tol += 2 * N_PEAKED * 2.0 ** -35 * vmax
+    tol += 2 * N_PEAKED * 2.0 ** (-32 if many else -35) * vmax
     tol += (2.0 ** -8 if bf16 else 2.0 ** -11) * (np.abs(ref) + tol) + 2.0 ** -25
     over = np.abs(got - ref) / tol
     at = np.unravel_index(over.argmax(), over.shape)
     assert over.max() <= 1, (at, got[at], ref[at[1:]], over.max())
+
+
+# ---- long stretches walked by one CTA ---------------------------------------------
+
+@pytest.mark.parametrize("keys", ["random", "flat"])
+@pytest.mark.parametrize("out_type", [TYPE_F16, TYPE_BF16])
+@pytest.mark.parametrize("tokens,heads", [(5, 4), (40, 4)])
+def test_long_items_do_not_shrink(ctx, tokens, heads, out_type, keys):
+    """More items of 1024 key tiles than SMs: one CTA sums most of an item.  What each addition
+    cuts off (or rounds in one direction, where all weights are alike) must not add up."""
+    rng = np.random.default_rng(tokens)
+    batch, n = 160, 131072
+    v = (1 + rng.random(R.D) + 0.3 * rng.standard_normal((n, R.D))).astype(np.float32)
+    if keys == "random":
+        k = rng.standard_normal((n, R.D)).astype(np.float32)
+        q = 1.2 * rng.standard_normal((1, tokens, heads, R.D))
+    else:  # one key above all the others, by a fraction of an octave
+        k = np.repeat(rng.standard_normal((1, R.D)), n, axis=0).astype(np.float32)
+        k[:, 0] = 0
+        k[0, 0] = 8
+        q = np.zeros((1, tokens, heads, R.D))
+        q[..., 0] = rng.uniform(0.2, 0.9, (tokens, heads)) * np.log(2) * np.sqrt(R.D) / 8
+    q = q.astype(np.float16)
+    k_rows, v_rows = R.quantize(k), R.quantize(v)
+    got = _attend(ctx, k_rows, v_rows, batch, np.repeat(q, batch, axis=0), out_type)
+
+    kv, vv = R.values(k_rows), R.values(v_rows)
+    ref = np.empty((tokens, heads, R.D))
+    for t in range(tokens):
+        s = q[0, t].astype(np.float64) @ kv[:n - tokens + t + 1].T / np.sqrt(R.D)
+        p = np.exp(s - s.max(1, keepdims=True))
+        ref[t] = p @ vv[:len(s[0])] / p.sum(1, keepdims=True)
+    eps = 2.0 ** -10 if out_type == TYPE_F16 else 2.0 ** -7
+    # half a step of rounding, uniform, in the mean square; operands rounded to fp16 for bf16 outputs
+    bound = eps / 2 / 3 ** .5 + 3e-5 + (9 * 2.0 ** -11 / 3 ** .5 if out_type == TYPE_BF16 else 0)
+    assert np.linalg.norm(got - ref) / (batch ** .5 * np.linalg.norm(ref)) < bound
+    if out_type == TYPE_F16:
+        # The mean over a head's outputs, whose own roundings cancel: four deviations of their mean.  A sum
+        # of 128 key tiles takes 24 products each, every one cutting off at most 2^-23 of what is there,
+        # half of the sum on average: 1.84e-4.
+        bias = (got / ref - 1).mean((1, 3))  # [batch][heads]
+        assert np.abs(bias).max() < 1.84e-4 + 4 * eps / 2 / 3 ** .5 / (tokens * R.D) ** .5
