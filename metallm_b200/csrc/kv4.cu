@@ -16,8 +16,7 @@
 // 43 MB, take 14.5 us in a graph, one token 3.1 us.
 #include <algorithm>
 
-#include "mlm_device.cuh"
-#include "mlm_internal.h"
+#include "kv4_common.cuh"
 
 // Pointers carry no __restrict__: their data may come from the kernel this one
 // is a programmatic dependent of, so no load may move above the dependent wait,
@@ -128,12 +127,12 @@ __device__ __forceinline__ bool row_at(int n_kv, int tokens, int capacity, const
   const int first = pos[b];
   if (counts) {
     const int n = counts[b];
-    if ((n < 0 || n > tokens) && t == 0 && report) *status = MLM_ERR_SHAPE;
+    if ((n < 0 || n > tokens) && t == 0 && report) report_outside(status);
     if (t >= n) return false;
   }
   const long long slot = (long long)first + t;
   if (slot < 0 || slot >= capacity) {
-    if (report) *status = MLM_ERR_SHAPE;
+    if (report) report_outside(status);
     return false;
   }
   r.source_row = (size_t)b * tokens + t;

@@ -294,8 +294,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
         int len, count;
         seq_shape(a, b, len, count);
         n = count > 0 ? (len + kBlk - 1) / kBlk * a.n_kv : 0;
-        if (blockIdx.x == 0 && seq_outside(a, b))
-          *a.status = MLM_ERR_SHAPE;
+        if (blockIdx.x == 0 && seq_outside(a, b)) report_outside(a.status);
       }
       int in = n;
 #pragma unroll

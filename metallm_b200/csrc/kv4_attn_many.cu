@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(Kv4AttnArgs 
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     if (lane == 0) {
       s_off[b + 1] = n;
-      if (blockIdx.x == 0 && seq_outside(a, b)) *a.status = MLM_ERR_SHAPE;
+      if (blockIdx.x == 0 && seq_outside(a, b)) report_outside(a.status);
     }
   }
   tc_fence_before();

@@ -1,5 +1,5 @@
-// kv4_common.cuh -- what the kernels of the attention over the 4-bit KV cache
-// share: the sequences' shapes as read from device memory, small conversions.
+// kv4_common.cuh -- what the kernels on the 4-bit KV cache share: the sequences' shapes as
+// read from device memory, the report of a bad one, small conversions.
 #pragma once
 
 #include "mlm_device.cuh"
@@ -35,6 +35,10 @@ __device__ __forceinline__ bool seq_outside(const Kv4AttnArgs &a, int b) {
   return a.lens[b] < 0 || a.lens[b] > a.capacity ||
          (a.counts && (a.counts[b] < 0 || a.counts[b] > a.tokens));
 }
+
+// a position, length or count outside its cache, unless the word already tells of a worse
+// failure (a wait that ran out)
+__device__ __forceinline__ void report_outside(int *status) { atomicCAS(status, 0, MLM_ERR_SHAPE); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
