@@ -454,7 +454,9 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_few_kernel(Kv4AttnArgs a) 
         }
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        // the largest |q| of the row into [2^13, 2^14): q / 16 keeps its bits
+        // the largest |q| of the row into [2^13, 2^14): q / 16 keeps its bits (an infinite one
+        // as the largest finite, so that cs stays a positive number)
+        big = fminf(big, 65504.f);
         const int e = big > 0.f ? 13 - ((int)((__float_as_uint(big) >> 23) & 0xFF) - 127) : 0;
         const float up = __uint_as_float((uint32_t)(e + 127) << 23);
         cs[nt] = kInvSqrtD * kLog2e * __uint_as_float((uint32_t)(24 - e + 127) << 23);

@@ -142,3 +142,18 @@ def test_long_items_do_not_shrink(ctx, tokens, heads, out_type, keys):
         # half of the sum on average: 1.84e-4.
         bias = (got / ref - 1).mean((1, 3))  # [batch][heads]
         assert np.abs(bias).max() < 1.84e-4 + 4 * eps / 2 / 3 ** .5 / (tokens * R.D) ** .5
+
+
+# ---- infinities in queries ----------------------------------------------------------
+
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan, 65504.0])
+@pytest.mark.parametrize("tokens,heads", [(2, 2), (4, 2), (8, 2), (20, 2)])
+def test_a_token_that_sees_nothing_gives_zeros_whatever_its_query(ctx, tokens, heads, value):
+    """Two rows cached: all but the last two tokens see none of them."""
+    rng = np.random.default_rng(tokens)
+    q = rng.standard_normal((1, tokens + 2, heads, R.D)).astype(np.float16)
+    q[0, :tokens, 0, 5] = value
+    k, v = (R.quantize(rng.standard_normal((2, R.D)).astype(np.float32)) for _ in "kv")
+    got = _attend(ctx, k, v, 1, q, TYPE_F16)
+    assert np.all(got[0, :tokens] == 0)
+    assert np.all(np.isfinite(got[0, tokens:]))
