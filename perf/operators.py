@@ -293,22 +293,26 @@ def _sample(s):
 
 # ---- the framework's calls --------------------------------------------------
 
-_context = []
+_contexts = {}  # of each device: the package, the context, the stream it is on
 
 
-def _own_context():
-    """The program's one context, on torch's current stream."""
-    if not _context:
+def _own_context(device):
+    """The program's context of a device, on torch's current stream there (asked for as a raw
+    handle: a Stream object takes 1 to 3 us to make)."""
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    at = _contexts.get(device)
+    if at is None:
         import metallm_b200
-        ctx = metallm_b200.Context(torch.cuda.current_device())
-        ctx.set_stream(torch.cuda.current_stream().cuda_stream or 1)  # 1: the default stream's handle
-        _context.append((metallm_b200, ctx))
-    return _context[0]
+        at = _contexts[device] = [metallm_b200, metallm_b200.Context(device), None]
+    if at[2] != stream:
+        at[1].set_stream(stream or 1)  # 1: the default stream's handle
+        at[2] = stream
+    return at
 
 
 def _own(s):
-    M, ctx = _own_context()
     c = s["case"]
+    M, ctx, _ = _own_context((s["token"] if c["op"] == "sample" else s["cache"][0]).get_device())
     if c["op"] == "sample":
         ctx.sample_f32(s["logits"].data_ptr(), c["rows"], c["n"], c["n"], s["params"].data_ptr(), s["u"].data_ptr(),
                        s["token"].data_ptr(), s["prob"].data_ptr())
