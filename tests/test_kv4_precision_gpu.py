@@ -1,5 +1,5 @@
 """Attention over the 4-bit cache where its precision is at stake: small weights beside large
-ones, long stretches of a cache walked by one CTA."""
+ones, long stretches of a cache walked by one CTA, sharp scores."""
 from __future__ import annotations
 
 import numpy as np
@@ -157,3 +157,21 @@ def test_a_token_that_sees_nothing_gives_zeros_whatever_its_query(ctx, tokens, h
     got = _attend(ctx, k, v, 1, q, TYPE_F16)
     assert np.all(got[0, :tokens] == 0)
     assert np.all(np.isfinite(got[0, tokens:]))
+
+
+# ---- sharp scores --------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens,heads", [(3, 4), (2, 8), (4, 4), (40, 4)])
+@pytest.mark.parametrize("out_type", [TYPE_F16, TYPE_BF16])
+@pytest.mark.parametrize("q_scale", [0.0, 1e-4, 8.0, 60.0])
+def test_sharp_and_flat_scores_to_their_own_precision(ctx, tokens, heads, out_type, q_scale):
+    """Each output type against the operands that it takes: an fp16 output's are never rounded alone."""
+    rng = np.random.default_rng(9)
+    n = 200
+    k, v = (R.quantize(rng.standard_normal((n, R.D)).astype(np.float32)) for _ in "kv")
+    q = (q_scale * rng.standard_normal((1, tokens, heads, R.D))).astype(np.float16)
+    got = _attend(ctx, k, v, 1, q, out_type)
+    ref, smax, vmax = R.attention(q, k[None, None], v[None, None], [n], [tokens])
+    bf16, many = out_type == TYPE_BF16, tokens * heads > 16
+    tol = R.attention_tolerance(ref, smax, vmax, 2.0 ** -7 if bf16 else 2.0 ** -10, bf16 and many, bf16 and not many)
+    assert np.all(np.abs(got - ref) <= tol), np.max(np.abs(got - ref) / tol)
