@@ -379,7 +379,9 @@ int mlm_attn_decode(mlm_ctx *ctx, const void *q_f16, const void *k_cache_f16,
  * device memory, so a captured graph can be replayed while they grow.  Values
  * outside the cache do not fault: rows beyond the capacity are skipped,
  * lengths and counts are kept within their range, and mlm_wait reports
- * MLM_ERR_SHAPE.
+ * MLM_ERR_SHAPE.  (The library's own rotations, mlm_rope_f16 and
+ * mlm_rope_qk_kv_append, take the position from the host: a captured step
+ * rotates its queries and keys by a kernel of the caller's.)
  * ------------------------------------------------------------------------ */
 
 #define MLM_KV4_ROW_BYTES 80
@@ -425,10 +427,12 @@ int mlm_kv4_read_f16(mlm_ctx *ctx, const mlm_kv4_cache *cache, int tokens, const
  * token that attends to no row gets zeros; out rows at and past counts_dev[b]
  * are left as they were.  q fp16 and out (out_type MLM_TYPE_F16 or BF16)
  * [batch][tokens][n_heads][128], 16-byte aligned; n_heads a multiple of
- * n_kv_heads.  Scores, softmax statistics and sums are fp32; an fp16 output is
- * within its own rounding of the exact one, as a rule; for a bf16 output V's
- * scaled weights, and with more than 16 (token, head) rows per KV head K, V and
- * the weights, are rounded to fp16 once.  A NaN in a key or value row reaches
+ * n_kv_heads.  Scores, softmax statistics and sums are fp32, and a weight is
+ * held to 2^-35 of the largest (2^-32 with more than 16 (token, head) rows per KV
+ * head).  An fp16 output is within its own rounding of the exact one, as a rule.
+ * For a bf16 output the weights are rounded to fp16, and their products with V's
+ * scales once more; with more than 16 rows per KV head K, V and the weights are,
+ * once each.  A NaN in a key or value row reaches
  * every token that sees the row, in its own dimensions or in all of them, and
  * no other token.  Uses
  * the context's attention scratch (39 MB): launches on one context are

@@ -19,8 +19,8 @@ constexpr int kD = kKv4D;
 
 // ---------------------------------------------------------------------------
 // Few rows: up to 16 (token, head) pairs of one KV head at once -- a decode
-// step, a few drafted tokens.  Bound by the cache's bytes (160 per position
-// and KV head), then by instruction issue.
+// step, a few drafted tokens.  The floor is the cache's bytes (160 per position
+// and KV head).
 //
 // Both products run on the tensor cores on the codes themselves.  A masked
 // nibble in a binary16's low mantissa bits is the subnormal c 2^-24 (16 c
@@ -32,9 +32,10 @@ constexpr int kD = kKv4D;
 // B; V^T is the A operand (16 dimensions x 16 rows; ldmatrix.trans of the codes
 // as 16-bit units hands a lane the nibbles of two neighbouring rows side by
 // side), the weights p d the 8 columns of B.  Nothing of K or V is rounded; q is
-// fp16 already (scaled by a power of two per row, so that q / 16 stays exact);
-// p d goes in as fp16 hi + lo.  With at most four columns the hi and lo parts
-// share the eight columns of one product.  Scores, statistics and sums are fp32.
+// fp16 already (scaled by a power of two per row, so that q / 16 stays exact).  For an
+// fp16 output p and p d go in as fp16 hi + lo, and with at most four columns the hi and
+// lo parts share the eight columns of one product; for a bf16 output p is rounded to fp16
+// and p d once more.  Scores, statistics and sums are fp32.
 //
 // Work is cut by bytes, not by head: the blocks of 32 rows of every (sequence,
 // KV head) form one line, cut into equal stretches per CTA and again per warp
@@ -45,12 +46,16 @@ constexpr int kD = kKv4D;
 // pieces by their CTA, the CTAs' through the context's scratch by the last CTA of the
 // head to arrive, so sums do not depend on timing.
 //
-// Measured in a graph: 64 sequences x 8192 rows x 8 KV heads (673 MB) 117 us, 5.75 TB/s;
-// 131071 rows x 8 (168 MB) 44 us; 2048 rows 10 us, some 5 us of it the cut, the first
-// copies and the joins.  711 instructions per block of 32 rows, issue slots 60 % and the
-// ALU pipe (masks, transposes, conversions) 54 % busy on 24 ragged sequences.  Warps,
-// ring: 16 x 2 stages for 8 columns, 8 x 4 for 16 (the reverse: 139 us for the 64
-// sequences, 58 against 38 us for 8 x 4 tokens).
+// Measured: 64 sequences x 8192 rows x 8 KV heads (673 MB) 117 us, 5.75 TB/s (139 us once
+// a second of such calls has the card at its power limit, 1660 MHz for 1965); 131071 rows
+// x 8 (168 MB) 45 us; 2048 rows 10 us, some 5 us of it the cut, the first copies and the
+// joins.  On 24 ragged sequences no unit is full: issue slots 60 %, the ALU pipe (masks,
+// transposes, conversions) 53 %, DRAM 48 %; 718 instructions per block of 32 rows in four
+// warps per scheduler, each a chain from the copy to the second product.  128 registers
+// hold the body of 8 columns but for 32 to 40 bytes.  Sixteen columns take 1350
+// instructions per block in two warps per scheduler, issue slots 32 %: 8 x 4 tokens at
+// 4099 rows 39 us.  Warps, ring: 16 x 2 stages for 8 columns, 8 x 4 for 16 (the reverse:
+// 139 us for the 64 sequences, 58 against 38 us for 8 x 4 tokens).
 // ---------------------------------------------------------------------------
 
 constexpr int kBlk = 32;                     // cache rows per block

@@ -37,11 +37,13 @@
 // that several CTAs share leaves fp32 parts in the context's scratch, which a
 // second kernel joins in order.
 //
-// Measured in a graph: 1024 tokens at 8192, 32/8 heads, 148 us, 870 TFLOP/s, the tensor
-// pipe 44 % active: bound by the chain S, softmax, P, P V of the two row tiles (144 us
-// without exponentials, maxima and dequantization, 107 us without the products).  Half
-// tiles with a thread per row tile issuing took 167 us, handing P over in halves 170,
-// the maximum in a pass before the exponentials 164.  To fp16: 333 us.
+// Measured: 1024 tokens at 8192, 32/8 heads, 147 us, 877 TFLOP/s (162 us at the card's
+// power limit, 1810 MHz for 1965), the tensor pipe 44 % active: bound by the chain S,
+// softmax, P, P V of the two row tiles (144 us without exponentials, maxima and
+// dequantization, 107 us without the products).  At 96 registers a thread at launch the
+// kernel spills 350 bytes a thread (480 for fp16 outputs).  Half tiles with a thread per
+// row tile issuing took 167 us, handing P over in halves 170, the maximum in a pass
+// before the exponentials 164.  To fp16: 338 us.
 //
 // A NaN in a cache row reaches every token that sees the row and no other: a
 // masked weight is 0, but 0 x NaN is not, so a value row with NaN scales goes in

@@ -22,10 +22,10 @@
 //    distinct;
 //  - the draw is by index: masses per warp's stretch of the row, a scan, and the
 //    one stretch that holds the point is walked again by the whole CTA.
-// Bound by the latency of these steps for few rows and by instruction issue (the fp64
-// exponentials of rows whose whole mass counts) for many: one row of 128256 tokens with
-// a top-k of 40 12.4 us in a graph, 64 rows of mixed settings 56 us, with top-p alone
-// about 100 us; their bytes would take 0.1 and 5 us.
+// Bound by the latency of these steps: one row of 128256 tokens with a top-k of 40 12.4
+// us, 64 rows of mixed settings 56 to 71 us (by their values), with top-p alone 101 us;
+// their bytes would take 0.1 and 5 us.  With 64 rows issue slots are 51 to 54 % busy, the
+// ALU pipe a third, the fp64 pipe 11 %; the 256 CTAs, one per SM, take 1.7 waves.
 // One cluster of CTAs per row; a CTA keeps its slice of the row in shared memory
 // (read once) where it fits and reads it again from L2 where it does not.
 #include <cooperative_groups.h>
